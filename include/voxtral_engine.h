@@ -7,7 +7,8 @@
  * 26-layer backbone decode step and the flow-matching CFG Euler loop.  Every
  * entry point below names the reference method it stands in for.  Plain C
  * types only: host arrays are copied in and out; the engine owns all device
- * memory.
+ * memory.  (The operators for batches, at the end, work on the caller's
+ * device memory instead.)
  *
  * Conventions
  *   - Every function returning int returns VX_OK (0) or a negative VX_E*
@@ -340,6 +341,134 @@ int vx_sample_top_p(vx_engine *e, const float *logits, int32_t n, int32_t valid,
 int vx_sample_top_p_noalloc(const float *logits, int32_t n, int32_t valid,
                             double top_p, double temperature, uint64_t *state,
                             uint32_t *code);
+
+/* ------------------------------------------- batches on device memory */
+/* No counterparts in the reference, which decodes one sequence: the cache,
+ * the attention and the sampling of a batch that decodes together, for
+ * callers whose data is on the GPU.  Unlike the engine's calls, these take
+ * device pointers of the GPU `device` (hipMalloc, a framework's tensors),
+ * enqueue their kernels on `stream` (a hipStream_t of that GPU; NULL: the
+ * null stream) and return without waiting.  They keep nothing between calls
+ * and allocate nothing, so they can be captured into graphs and called from
+ * several threads; calls that write the same memory must be ordered by the
+ * caller.  What they need beside their operands is the caller's workspace:
+ * its contents are free to change between calls, and two calls that may run
+ * at the same time (two graphs, two streams) need one each.
+ * Strides count elements; the last dimension is contiguous.  Rows and caches
+ * must be aligned to 16 bytes, strides included.  Errors: VX_E_*, the message
+ * by vx_batch_error() on the calling thread.  Host checks see sizes only.
+ * Ids, lengths and row starts are read on the GPU and tested there: what lies
+ * outside its pool or bound counts as absent, and no access is made with it. */
+#define VX_TYPE_F32 0
+#define VX_TYPE_F16 1
+#define VX_TYPE_BF16 2
+
+/* The last failed batch call's message of the calling thread. */
+const char *vx_batch_error(void);
+
+/* K and V pools [page][kv head][slot][head_dim], the same strides for both.
+ * page_size: a power of two, 16..4096; head_dim 64 or 128.  Rows (k, v, q,
+ * out) are of the cache's type, or f32 for an f16 cache. */
+typedef struct vx_paged_kv {
+  void *k, *v;
+  int64_t page_stride, head_stride, token_stride;
+  int32_t n_pages, page_size, n_kv_heads, head_dim;
+  int32_t type; /* VX_TYPE_* */
+  int32_t device;
+} vx_paged_kv;
+
+/* Appends keys and values, turned by their positions on the way: the batch
+ * form of what the QKV product's epilogue does with rope and kvCacheWrite
+ * (src/shaders.ts:224-256, 452-473).  Token t of sequence s = seq[t] (NULL:
+ * t) at position pos[t] goes to slot pos[t] - base of the sequence, which is
+ * slot (pos - base) mod page_size of page table[s][(pos - base) / page_size].
+ * base: the positions that a shared prefix takes.  In K and Q the pairs of
+ * the first rotary_dim elements (a multiple of 16; 0: none) turn by pos
+ * theta^(-2 i / rotary_dim), pairs (2 i, 2 i + 1) if interleaved, else
+ * (i, i + rotary_dim / 2); angles are formed in 64 bits.  q (nullable) is
+ * turned into q_out, which may be q.  A token is skipped, its q too, where
+ * pos < 0, seq is not in [0, n_seqs), or its slot has no page.  Two tokens of
+ * a call must not name the same slot: either's elements may be found there. */
+typedef struct vx_append_args {
+  vx_paged_kv kv;
+  const void *k, *v;                       /* [n_tokens][n_kv_heads][head_dim] */
+  int64_t k_row, k_head, v_row, v_head;
+  const void *q;                           /* [n_tokens][n_heads][head_dim] or NULL */
+  void *q_out;
+  int64_t q_row, q_head, o_row, o_head;
+  const int32_t *pos, *seq;                /* [n_tokens] */
+  const int32_t *table;                    /* [n_seqs][table_width] */
+  int64_t table_stride;
+  int32_t table_width, base, n_tokens, n_seqs, n_heads;
+  int32_t type;                            /* of k, v, q */
+  double theta;
+  int32_t rotary_dim, interleaved;
+} vx_append_args;
+int vx_paged_append(const vx_append_args *a, void *stream);
+
+/* Attention of a batch whose sequences share a prefix: the batch form of the
+ * decode step's (src/shaders.ts:306-447).  Query rows row_start[s] ..
+ * row_start[s + 1] - 1 are sequence s's last ones (NULL: one row each).  The
+ * j-th of its n rows sees the prefix_len keys of prefix_pages and the first
+ * min(lens[s] - (n - 1 - j), max_len) keys of the sequence's own pages:
+ * out = softmax(scale q K^T) V over all of them, query head h reading KV head
+ * h / (n_heads / n_kv_heads).  scale 0: 1 / sqrt(head_dim).  A row that sees
+ * no key gets zeros, and lse = -inf; rows from row_start[n_seqs] on are left
+ * as they are.  lse (nullable): [n_rows][n_heads], the logarithm of the sum
+ * of exponentials.  max_len: a bound on lens that the host knows, at most
+ * table_width * page_size; work is dealt out by it.  Scores, softmax and sums
+ * are f32; with 16-bit rows the weights are rounded to the cache's type
+ * before they meet the values. */
+typedef struct vx_attend_args {
+  vx_paged_kv kv;
+  const void *q;                           /* [n_rows][n_heads][head_dim] */
+  void *out;
+  float *lse;
+  int64_t q_row, q_head, o_row, o_head;
+  const int32_t *row_start;                /* [n_seqs + 1] or NULL */
+  const int32_t *lens;                     /* [n_seqs] */
+  const int32_t *table;                    /* [n_seqs][table_width] */
+  const int32_t *prefix_pages;             /* [prefix_count] */
+  int64_t table_stride;
+  int32_t table_width, prefix_count, prefix_len, max_len;
+  int32_t n_rows, n_seqs, n_heads;
+  int32_t type;                            /* of q, out */
+  float scale;
+  void *workspace;                         /* aligned to 16 bytes */
+  size_t workspace_bytes;
+} vx_attend_args;
+int vx_paged_attend(const vx_attend_args *a, void *stream);
+/* The bytes of workspace that a call with these sizes needs (pointers are not
+ * read; row_start only for being NULL or not). */
+int vx_paged_attend_workspace(const vx_attend_args *a, size_t *bytes);
+
+/* Draws a token for each row of logits from given uniforms: the batch form
+ * of vx_sample_top_p, for any vocabulary of up to 2^20 and with top-k and
+ * min-p beside top-p.  Order: logit descending, index ascending; NaN and -inf
+ * are never drawn.  With weights exp((x - max) / temperature), kept is the
+ * shortest of three prefixes of the order, at least one entry: top_k entries
+ * (0: all); the first whose weights reach top_p of the top-k entries' (1:
+ * all); the entries whose weight is at least min_p (0: all; the maximum's
+ * weight is 1).  token: the first entry of the order whose running sum passes
+ * u times the kept sum, u in [0, 1); temperature 0 or less: the first entry.
+ * Weights are rounded to 2^-43 and summed exactly, so results do not depend
+ * on the order of sums.  kept and prob (nullable) receive the number of kept
+ * entries and the drawn one's share of their weights.  A row with nothing to
+ * draw gives token -1, kept 0, prob 0.  Each of temperature, top_k, top_p,
+ * min_p is [rows] on the device, or NULL for the same value in every row. */
+typedef struct vx_sample_args {
+  const void *logits;                      /* [rows][n] */
+  int64_t row_stride;
+  const float *temperature, *top_p, *min_p;
+  const int32_t *top_k;
+  const double *u;                         /* [rows] */
+  int32_t *token, *kept;
+  float *prob;
+  int32_t rows, n, type, device;
+  float temperature0, top_p0, min_p0;
+  int32_t top_k0;
+} vx_sample_args;
+int vx_sample_rows(const vx_sample_args *a, void *stream);
 
 /* ------------------------------------------------------ measurement */
 /* No reference counterparts (the reference times on the CPU,

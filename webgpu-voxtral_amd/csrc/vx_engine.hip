@@ -25,6 +25,7 @@
 #include "vx_stage.h"
 #include "vx_loader.h"
 #include "vx_tokenizer.h"
+#include "vx_batch.h"
 
 #include <fcntl.h>
 #include <unistd.h>
@@ -2500,5 +2501,23 @@ int vx_time_kernel(vx_engine *e, int32_t kernel, int32_t iters, float *avg_us, d
   *avg_us = ms * 1000.0f / iters;
   return VX_OK;
 }
+
+// ------------------------------------- batches on the caller's memory
+const char *vx_batch_error(void) { return batch_error(); }
+
+int vx_paged_append(const vx_append_args *a, void *stream) { return paged_append(a, stream); }
+
+int vx_paged_attend(const vx_attend_args *a, void *stream) { return paged_attend(a, stream); }
+
+int vx_paged_attend_workspace(const vx_attend_args *a, size_t *bytes) {
+  if (!bytes) return batch_fail(VX_E_INVALID, "vx_paged_attend_workspace: NULL argument");
+  PagedKV kv;
+  AttendPlan plan;
+  if (int rc = check_attend("vx_paged_attend_workspace", a, &kv, &plan)) return rc;
+  *bytes = plan.bytes;
+  return VX_OK;
+}
+
+int vx_sample_rows(const vx_sample_args *a, void *stream) { return sample_rows(a, stream); }
 
 }  // extern "C"

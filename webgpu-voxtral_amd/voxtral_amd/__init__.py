@@ -128,6 +128,12 @@ _SIGS = {
                               ctypes.POINTER(ctypes.c_double)]),
     "vx_debug_timeline": (_I32, [_VP, _I32, _VP, _I32, ctypes.POINTER(_I32)]),
     "vx_synchronize": (_I32, [_VP]),
+    # batches on device memory: an argument structure's bytes, the stream
+    "vx_batch_error": (ctypes.c_char_p, []),
+    "vx_paged_append": (_I32, [ctypes.c_char_p, _VP]),
+    "vx_paged_attend": (_I32, [ctypes.c_char_p, _VP]),
+    "vx_paged_attend_workspace": (_I32, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_size_t)]),
+    "vx_sample_rows": (_I32, [ctypes.c_char_p, _VP]),
 }
 
 _lib = None
@@ -568,3 +574,7 @@ class VoxtralEngine:
 
     def synchronize(self):
         self._check(self._lib.vx_synchronize(self._h))
+
+
+# the operators for batches on GPU tensors (torch is imported by their first use)
+from .batch import PagedKV, sample_rows  # noqa: E402,F401

@@ -1,0 +1,257 @@
+"""Operators for batches that decode together, on tensors in GPU memory
+(vx_paged_append, vx_paged_attend and vx_sample_rows of
+include/voxtral_engine.h): a paged key/value cache, the attention of a batch
+that shares a prefix, and sampling.
+
+Arguments are torch tensors of one GPU.  Calls are enqueued on the stream that
+is current for it (`stream`: another one, an object with `cuda_stream` or its
+number; the tensors must then be kept alive, and ready, for that stream by the
+caller) and return without waiting.  They can be captured into graphs.  Wrong
+shapes, types, strides or devices raise ValueError or TypeError, what the
+library refuses raises VoxtralError.  There is no backward pass: tensors that
+require gradients are refused while gradients are recorded."""
+import ctypes
+import struct
+
+from . import VX_OK, VoxtralError, load_library
+
+# the argument structures of the C ABI, in native layout
+_KV = struct.Struct("@PPqqqiiiiii")
+_APPEND = struct.Struct("@64sPPqqqqPPqqqqPPPqiiiiiidii")
+_ATTEND = struct.Struct("@64sPPPqqqqPPPPqiiiiiiiif4xPN")
+_SAMPLE = struct.Struct("@PqPPPPPPPPiiiifffi")
+assert _KV.size == 64
+
+_torch = None
+_types = None  # dtype -> VX_TYPE_*
+
+
+def _load():
+    global _torch, _types
+    if _torch is None:
+        import torch
+        _types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+        _torch = torch
+    return load_library()
+
+
+def _call(fn, *args):
+    rc = fn(*args)
+    if rc != VX_OK:
+        raise VoxtralError(rc, load_library().vx_batch_error().decode())
+
+
+def _stream(device, stream):
+    if stream is None:
+        return _torch.cuda.current_stream(device).cuda_stream
+    return getattr(stream, "cuda_stream", stream)
+
+
+def _tensor(name, x, dims, device):
+    """x checked: a tensor of `dims` dimensions on `device`, its last one contiguous."""
+    if not isinstance(x, _torch.Tensor):
+        raise TypeError(f"{name}: a torch tensor is needed, not {type(x).__name__}")
+    if x.device != device or device.type != "cuda":
+        raise ValueError(f"{name} is on {x.device}, not on the GPU {device}")
+    if x.dim() != dims:
+        raise ValueError(f"{name} has {x.dim()} dimensions, not {dims}")
+    if x.shape[-1] > 1 and x.stride(-1) != 1:
+        raise ValueError(f"{name}: the last dimension is not contiguous")
+    if x.requires_grad and _torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient: this operator has no backward pass")
+    return x
+
+
+def _ints(name, x, n, device):
+    """The address of a contiguous int32 vector of n elements."""
+    _tensor(name, x, 1, device)
+    if x.dtype != _torch.int32:
+        raise TypeError(f"{name}: int32 is needed, not {x.dtype}")
+    if n is not None and x.shape[0] != n:
+        raise ValueError(f"{name} has {x.shape[0]} elements, not {n}")
+    return x.data_ptr()
+
+
+class PagedKV:
+    """A paged cache of one layer: K and V pools [page][kv head][slot][head_dim]
+    of float32, float16 or bfloat16, with the same strides.  A sequence's slot
+    s is slot s mod page_size of page table[sequence][s // page_size]; which
+    pages belong to which sequence is the caller's.  Rows (q, k, v, out) are of
+    the pools' type, or float32 for float16 pools."""
+
+    def __init__(self, k_pages, v_pages):
+        self._lib = _load()
+        self.device = getattr(k_pages, "device", None)
+        _tensor("k_pages", k_pages, 4, self.device)
+        _tensor("v_pages", v_pages, 4, self.device)
+        if v_pages.shape != k_pages.shape or v_pages.stride() != k_pages.stride() or v_pages.dtype != k_pages.dtype:
+            raise ValueError("k_pages and v_pages differ in shape, strides or type")
+        if k_pages.dtype not in _types:
+            raise TypeError(f"k_pages: float32, float16 or bfloat16 is needed, not {k_pages.dtype}")
+        self.k_pages, self.v_pages = k_pages, v_pages
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k_pages.shape
+        self._head = _KV.pack(k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], self.n_pages, self.page_size,
+                              self.n_kv_heads, self.head_dim, _types[k_pages.dtype], self.device.index or 0)
+
+    def _rows(self, name, x, tokens, heads):
+        _tensor(name, x, 3, self.device)
+        if x.dtype not in _types:
+            raise TypeError(f"{name}: float32, float16 or bfloat16 is needed, not {x.dtype}")
+        if x.shape[2] != self.head_dim or (tokens is not None and x.shape[0] != tokens) or (heads is not None and x.shape[1] != heads):
+            raise ValueError(f"{name} has shape {tuple(x.shape)}, not ({tokens}, {heads}, {self.head_dim})")
+        return x
+
+    def _table(self, table):
+        _tensor("table", table, 2, self.device)
+        if table.dtype != _torch.int32:
+            raise TypeError(f"table: int32 is needed, not {table.dtype}")
+        return table
+
+    def append(self, k, v, pos, table, seq=None, base=0, q=None, q_out=None, theta=1e6, rotary_dim=None, interleaved=True,
+               stream=None):
+        """Writes k and v [tokens][kv heads][head_dim] to the cache, k (and q,
+        into q_out) turned by their positions: token t of sequence seq[t]
+        (None: t) at position pos[t] goes to the sequence's slot pos[t] -
+        base.  rotary_dim: elements that turn (None: all; 0: none).  Tokens
+        with a negative pos, a seq outside the table or a slot without a page
+        are skipped.  Returns q_out (None without q; made, with zeros for
+        skipped tokens, if not given)."""
+        k = self._rows("k", k, None, self.n_kv_heads)
+        n = k.shape[0]
+        v = self._rows("v", v, n, self.n_kv_heads)
+        table = self._table(table)
+        if v.dtype != k.dtype:
+            raise TypeError(f"v is {v.dtype}, k is {k.dtype}")
+        heads, qs = 0, (0, 0, 0, 0, 0, 0)
+        if q is not None:
+            q = self._rows("q", q, n, None)
+            heads = q.shape[1]
+            if q_out is None:
+                q_out = q.new_zeros(q.shape)
+            else:
+                self._rows("q_out", q_out, n, heads)
+            if q.dtype != k.dtype or q_out.dtype != k.dtype:
+                raise TypeError(f"q is {q.dtype}, q_out is {q_out.dtype}, k is {k.dtype}")
+            qs = (q.data_ptr(), q_out.data_ptr(), q.stride(0), q.stride(1), q_out.stride(0), q_out.stride(1))
+        args = _APPEND.pack(self._head, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), *qs,
+                            _ints("pos", pos, n, self.device), 0 if seq is None else _ints("seq", seq, n, self.device),
+                            table.data_ptr(), table.stride(0), table.shape[1], base, n, table.shape[0], heads, _types[k.dtype],
+                            theta, self.head_dim if rotary_dim is None else rotary_dim, bool(interleaved))
+        _call(self._lib.vx_paged_append, args, _stream(self.device, stream))
+        return q_out if q is not None else None
+
+    def attend(self, q, lens, table, row_start=None, prefix_pages=None, prefix_len=0, max_len=None, scale=None, out=None,
+               lse=None, workspace=None, stream=None):
+        """Attention of a batch that shares a prefix.  q [rows][heads][head_dim]:
+        one row a sequence, or rows row_start[s] .. row_start[s + 1] - 1 for
+        sequence s, its last ones.  A row sees the prefix_len keys of
+        prefix_pages (page ids) and the first lens[s] keys of its sequence's
+        own pages, less one for each row of the sequence behind it.  max_len: a
+        bound on lens (None: what the table holds); keys from there on are not
+        seen.  scale None: 1 / sqrt(head_dim).  lse [rows][heads] float32
+        receives the logarithms of the sums of exponentials.  Returns out
+        (made if not given, with zeros in rows behind the last sequence).
+        workspace: a uint8 tensor of attend_workspace() bytes for this call
+        alone (None: made by this call)."""
+        q = self._rows("q", q, None, None)
+        n, heads = q.shape[0], q.shape[1]
+        table = self._table(table)
+        seqs, width = table.shape
+        lens_at = _ints("lens", lens, seqs, self.device)
+        start = 0 if row_start is None else _ints("row_start", row_start, seqs + 1, self.device)
+        pages, count = 0, 0
+        if prefix_pages is not None:
+            pages = _ints("prefix_pages", prefix_pages, None, self.device)
+            count = prefix_pages.shape[0]
+        if max_len is None:
+            max_len = width * self.page_size
+        if out is None:
+            out = q.new_empty(q.shape) if row_start is None else q.new_zeros(q.shape)
+        else:
+            self._rows("out", out, n, heads)
+            if out.dtype != q.dtype:
+                raise TypeError(f"out is {out.dtype}, q is {q.dtype}")
+        if lse is not None:
+            _tensor("lse", lse, 2, self.device)
+            if lse.dtype != _torch.float32 or lse.shape != (n, heads) or not lse.is_contiguous():
+                raise ValueError(f"lse: a contiguous float32 tensor of shape ({n}, {heads}) is needed")
+        if scale is None:
+            scale = 0.0
+        elif scale == 0:
+            raise ValueError("scale is 0")
+
+        def pack(at, size):
+            return _ATTEND.pack(self._head, q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), q.stride(0),
+                                q.stride(1), out.stride(0), out.stride(1), start, lens_at, table.data_ptr(), pages,
+                                table.stride(0), width, count, prefix_len, max_len, n, seqs, heads, _types[q.dtype], scale, at,
+                                size)
+
+        if workspace is None:
+            need = ctypes.c_size_t()
+            _call(self._lib.vx_paged_attend_workspace, pack(0, 0), ctypes.byref(need))
+            # on the stream's own terms: torch's allocator orders its reuse by the current stream
+            workspace = table.new_empty((need.value + 3) // 4)
+            if stream is not None and need.value:
+                workspace.record_stream(stream if isinstance(stream, _torch.cuda.Stream)
+                                        else _torch.cuda.ExternalStream(_stream(self.device, stream), self.device))
+        else:
+            _tensor("workspace", workspace, 1, self.device)
+        _call(self._lib.vx_paged_attend, pack(workspace.data_ptr(), workspace.numel() * workspace.element_size()),
+              _stream(self.device, stream))
+        return out
+
+    def attend_workspace(self, rows, heads, seqs, width, ragged=False, prefix_len=0, max_len=None, dtype=None):
+        """The bytes of workspace that attend() needs for `rows` query rows of
+        `heads` heads, a table of seqs x width pages and these bounds."""
+        need = ctypes.c_size_t()
+        t = _types[self.k_pages.dtype if dtype is None else dtype]
+        args = _ATTEND.pack(self._head, 0, 0, 0, 0, 0, 0, 0, int(ragged), 0, 0, 0, width, width,
+                            -(-prefix_len // self.page_size), prefix_len, width * self.page_size if max_len is None else max_len,
+                            rows, seqs, heads, t, 0.0, 0, 0)
+        _call(self._lib.vx_paged_attend_workspace, args, ctypes.byref(need))
+        return need.value
+
+
+def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, stream=None):
+    """Draws a token for each row of logits [rows][n] (float32, float16 or
+    bfloat16; n up to 2^20) by the uniforms u [rows] (float64, in [0, 1)):
+    among the top_k largest (0: all), the largest whose weights reach top_p of
+    those' (1: all), and the ones of at least min_p times the largest's weight,
+    weights being exp(logit / temperature).  The draw runs along the falling
+    logits, equal ones by index.  Each of temperature, top_k, top_p and min_p
+    is a number or a tensor [rows] (float32; int32 for top_k); temperature 0
+    takes the first of the largest.  Returns (token, kept, prob): int32 ids,
+    the numbers of tokens that were left to draw from, and the drawn one's
+    probability among them; a row with nothing but NaN and -inf gives (-1, 0,
+    0).  out: these three tensors, to write to."""
+    lib = _load()
+    device = getattr(logits, "device", None)
+    _tensor("logits", logits, 2, device)
+    if logits.dtype not in _types:
+        raise TypeError(f"logits: float32, float16 or bfloat16 is needed, not {logits.dtype}")
+    rows, n = logits.shape
+
+    def vector(name, x, dtype):
+        _tensor(name, x, 1, device)
+        if x.dtype != dtype:
+            raise TypeError(f"{name}: {dtype} is needed, not {x.dtype}")
+        if x.shape[0] != rows:
+            raise ValueError(f"{name} has {x.shape[0]} elements, not {rows}")
+        return x.data_ptr()
+
+    def setting(name, x, dtype):
+        return (vector(name, x, dtype), 0) if isinstance(x, _torch.Tensor) else (0, x)
+
+    f32, i32 = _torch.float32, _torch.int32
+    temperature, t0 = setting("temperature", temperature, f32)
+    top_k, k0 = setting("top_k", top_k, i32)
+    top_p, p0 = setting("top_p", top_p, f32)
+    min_p, m0 = setting("min_p", min_p, f32)
+    if out is None:
+        out = logits.new_empty(rows, dtype=i32), logits.new_empty(rows, dtype=i32), logits.new_empty(rows, dtype=f32)
+    token, kept, prob = out
+    _call(lib.vx_sample_rows,
+          _SAMPLE.pack(logits.data_ptr(), logits.stride(0), temperature, top_p, min_p, top_k, vector("u", u, _torch.float64),
+                       vector("token", token, i32), vector("kept", kept, i32), vector("prob", prob, f32), rows, n,
+                       _types[logits.dtype], device.index or 0, t0, p0, m0, k0), _stream(device, stream))
+    return token, kept, prob
