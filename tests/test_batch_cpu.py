@@ -85,8 +85,8 @@ def error():
     (lambda: attend(lens=0), "NULL argument"),
     (lambda: attend(prefix_pages=0), "NULL argument"),
     (lambda: attend(q_head=132), "multiples of 16"),
-    (lambda: attend(), "workspace of 0 bytes"),
-    (lambda: attend(workspace=P + 8, workspace_bytes=1 << 30), "aligned to 16"),
+    (lambda: attend(prefix_len=2000, prefix_count=125), "workspace of 0 bytes"),
+    (lambda: attend(prefix_len=2000, prefix_count=125, workspace=P + 8, workspace_bytes=1 << 30), "aligned to 16"),
     (lambda: sample(type=7), "type 7"),
     (lambda: sample(n=0), "0 logits"),
     (lambda: sample(n=(1 << 20) + 1), "more than"),
@@ -130,8 +130,9 @@ def test_errors_belong_to_their_thread():
 
 
 def test_workspace_covers_every_partial():
-    rc, n = attend(f="vx_paged_attend_workspace")
+    rc, n = attend(f="vx_paged_attend_workspace", prefix_len=2000, prefix_count=125)
     assert rc == V.VX_OK and n >= 2 * 3 * 32 * (128 + 2) * 4
+    assert attend(f="vx_paged_attend_workspace") == (V.VX_OK, 0)  # one split in all: no partials
     assert attend(f="vx_paged_attend_workspace", prefix_len=0, max_len=0) == (V.VX_OK, 0)
 
 
@@ -157,14 +158,19 @@ int main() {
             for (bool ragged : {false, true}) {
               const int seqs = ragged ? (r + 2) / 3 : r, g = h[0] / h[1];
               const AttendPlan p = attend_plan(r, seqs, h[0], h[1], hd, pre, len, ragged, 256);
-              if (pre && ((int64_t)p.pre_splits * p.pre_chunk < pre || (int64_t)(p.pre_splits - 1) * p.pre_chunk >= pre || p.pre_chunk % 32))
+              if (pre && !p.fused && ((int64_t)p.pre_splits * p.pre_chunk < pre || (int64_t)(p.pre_splits - 1) * p.pre_chunk >= pre ||
+                                      p.pre_chunk % 32 || (int64_t)p.pre_tiles * AT_COLS * p.pre_waves < (int64_t)r * g))
                 return 3;
-              if (len && ((int64_t)p.own_splits * p.own_chunk < len || (int64_t)(p.own_splits - 1) * p.own_chunk >= len || p.own_chunk % 32))
+              // a fused block's keys: the prefix in whole steps, then its own
+              const int64_t own = len + (p.fused ? at_ceil(pre, 32) * 32 : 0);
+              if (len && ((int64_t)p.own_splits * p.own_chunk < own || (int64_t)(p.own_splits - 1) * p.own_chunk >= own || p.own_chunk % 32))
                 return 4;
-              if (pre && (int64_t)p.pre_tiles * AT_COLS < (int64_t)r * g) return 5;
+              if (p.fused && (p.pre_splits || p.pre_tiles || !len)) return 5;
+              for (int w : {p.pre_waves, p.own_waves})
+                if (w != 1 && w != 2 && w != 4) return 9;
               if (p.blocks > 0x7fffffff || p.ml_at % 16) return 6;
               const size_t items = (size_t)(p.pre_splits + p.own_splits) * r * h[0];
-              if (p.bytes < items * (hd * 4 + 8) || p.ml_at < items * hd * 4) return 7;
+              if (!p.direct() && (p.bytes < items * (hd * 4 + 8) || p.ml_at < items * hd * 4)) return 7;
               if (!len) continue;
               // the slots of every sequence's tiles: distinct, in order, inside the grid
               std::vector<char> taken(p.own_slots, 0);
@@ -172,8 +178,8 @@ int main() {
               for (int s = 0; s < seqs; s++) {
                 const int n = !ragged ? 1 : s + 1 < seqs ? (s * 7) % 4 : r - r0;
                 const int r1 = r0 + n < r ? r0 + n : r;
-                const int tiles = (int)at_ceil((int64_t)(r1 - r0) * g, AT_COLS);
-                const int64_t first = ragged ? (int64_t)r0 * g / AT_COLS + s : (int64_t)s * at_ceil(g, AT_COLS);
+                const int tc = AT_COLS * p.own_waves, tiles = (int)at_ceil((int64_t)(r1 - r0) * g, tc);
+                const int64_t first = ragged ? (int64_t)r0 * g / tc + s : (int64_t)s * at_ceil(g, tc);
                 for (int t = 0; t < tiles; t++)
                   if (first + t >= p.own_slots || taken[first + t]++) return 8;
                 r0 = r1;

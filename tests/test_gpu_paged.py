@@ -331,12 +331,13 @@ def test_a_run_of_steps_streams_and_graphs():
 
 def test_a_given_workspace_and_stream():
     torch.manual_seed(16)
-    kp, vp = pools(40, 2, 16, 64, torch.bfloat16)
+    kp, vp = pools(240, 2, 16, 64, torch.bfloat16)
     kv = V.PagedKV(kp, vp)
-    table = torch.arange(40, dtype=torch.int32, device=DEV).view(4, 10)
-    q, lens = torch.randn(4, 4, 64, device=DEV).bfloat16(), ints([160, 3, 50, 100])
+    table = torch.arange(240, dtype=torch.int32, device=DEV).view(4, 60)
+    q, lens = torch.randn(4, 4, 64, device=DEV).bfloat16(), ints([960, 3, 50, 400])
     want = kv.attend(q, lens, table)
-    need = kv.attend_workspace(4, 4, 4, 10)
+    need = kv.attend_workspace(4, 4, 4, 60)
+    assert need > 0
     ws = torch.empty(need, dtype=torch.uint8, device=DEV)
     assert torch.equal(kv.attend(q, lens, table, workspace=ws), want)
     side = torch.cuda.Stream()

@@ -80,6 +80,7 @@ inline int check_kv(const char *what, const vx_paged_kv &kv, PagedKV *out) {
   if (kv.page_stride < 0 || kv.head_stride < 0 || kv.token_stride < kv.head_dim || !aligned16(kv.k, es, kv.page_stride, kv.head_stride) ||
       !aligned16(kv.v, es, kv.token_stride, 0))
     return batch_fail(VX_E_INVALID, "%s: the cache and its strides must be multiples of 16 bytes", what);
+  if (kv.token_stride > (1 << 24)) return batch_fail(VX_E_RANGE, "%s: token stride %lld", what, (long long)kv.token_stride);
   *out = PagedKV{kv.k, kv.v, kv.page_stride, kv.head_stride, kv.token_stride, kv.n_pages, kv.page_size,
                  31 - __builtin_clz((unsigned)kv.page_size), kv.n_kv_heads};
   return VX_OK;
@@ -183,8 +184,9 @@ inline int paged_attend(const vx_attend_args *p, void *stream) {
   a.prefix_len = p->prefix_len, a.max_len = p->max_len;
   a.n_rows = p->n_rows, a.n_seqs = p->n_seqs, a.n_heads = p->n_heads, a.group = p->n_heads / p->kv.n_kv_heads;
   a.scale = (p->scale == 0 ? 1.0f / sqrtf((float)p->kv.head_dim) : p->scale) * 1.4426950408889634f;
-  a.pre_tiles = plan.pre_tiles, a.pre_splits = plan.pre_splits, a.pre_chunk = plan.pre_chunk;
-  a.own_slots = plan.own_slots, a.own_splits = plan.own_splits, a.own_chunk = plan.own_chunk;
+  a.pre_waves = plan.pre_waves, a.pre_tiles = plan.pre_tiles, a.pre_splits = plan.pre_splits, a.pre_chunk = plan.pre_chunk;
+  a.own_waves = plan.own_waves, a.own_slots = plan.own_slots, a.own_splits = plan.own_splits, a.own_chunk = plan.own_chunk;
+  a.fused = plan.fused;
   a.part_o = (float *)p->workspace;
   a.part_ml = (float2 *)((char *)p->workspace + plan.ml_at);
   OnDevice on(p->kv.device);
@@ -192,7 +194,7 @@ inline int paged_attend(const vx_attend_args *p, void *stream) {
   return with_types(p->type, p->kv.type, [&](auto r, auto c) {
     auto go = [&](auto part, auto join) {
       int rc = plan.blocks ? batch_launch(what, part, plan.blocks, 64 * AT_WAVES, 0, a, stream) : VX_OK;
-      return rc ? rc : batch_launch(what, join, at_ceil((int64_t)a.n_rows * a.n_heads, 4), 256, 0, a, stream);
+      return rc || plan.direct() ? rc : batch_launch(what, join, at_ceil((int64_t)a.n_rows * a.n_heads, 4), 256, 0, a, stream);
     };
     using R = decltype(r);
     using C = decltype(c);

@@ -170,11 +170,12 @@ __global__ __launch_bounds__(PA_NT) void paged_append_kernel(AppendArgs a) {
 // Row r of sequence s, the j-th of its n_s rows: one softmax over the shared
 // prefix's keys and the first clamp(lens[s] - (n_s - 1 - j), 0, max_len) keys
 // of the sequence.  Columns: the n_s rows times the G query heads of a KV
-// head, row-major, 16 to a tile.  Blocks of the first kind take the prefix
-// with the columns of all rows, so its keys are read once for 16 columns and
-// not once a sequence; blocks of the second kind take a sequence's own keys.
-// Both split the key axis and leave (o, m, l) partials that a second kernel
-// joins.
+// head, row-major, 16 to a wave.  Blocks of the first kind take the prefix
+// with the columns of all rows, so its keys are read once for many columns
+// and not once a sequence; blocks of the second kind take a sequence's own
+// keys (and, where that is little, the prefix before them: `fused`).  Both
+// split the key axis and leave (o, m, l) partials that a second kernel joins,
+// unless there is one split in all.
 struct AttendArgs {
   PagedKV kv;
   const void *q;
@@ -186,51 +187,66 @@ struct AttendArgs {
   int table_width, prefix_count, prefix_len, max_len;
   int n_rows, n_seqs, n_heads, group;
   float scale;  // times log2(e)
-  // the plan: blocks of the prefix, splits and their keys (multiples of 32)
-  int pre_tiles, pre_splits, pre_chunk;
-  int own_slots, own_splits, own_chunk;
+  // the plan: column waves of a block, tiles of columns, splits and their
+  // keys (multiples of 32)
+  int pre_waves, pre_tiles, pre_splits, pre_chunk;
+  int own_waves, own_slots, own_splits, own_chunk;
+  int fused;
   float *part_o;   // [slot][row * heads + head][head_dim]
   float2 *part_ml; // [slot][row * heads + head]: maximum (log2 units), sum
 };
 
-constexpr int AT_COLS = 16;  // columns of a tile: the matrix instruction's
+constexpr int AT_COLS = 16;  // columns of a wave: the matrix instruction's
 constexpr int AT_KEYS = 32;  // keys of a wave's step: two tiles of 16
 constexpr int AT_WAVES = 4;
 
 struct AttendPlan {
-  int pre_tiles, pre_splits, pre_chunk, own_slots, own_splits, own_chunk;
+  int pre_waves, pre_tiles, pre_splits, pre_chunk, own_waves, own_slots, own_splits, own_chunk, fused;
   size_t ml_at, bytes;  // the workspace: part_o, then part_ml at ml_at
   int64_t blocks;
+  int slots() const { return pre_splits + own_splits; }
+  bool direct() const { return slots() == 1; }  // no partials: the blocks write the result
 };
 
 __host__ __device__ inline int64_t at_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Splits: enough blocks for about four on each compute unit, at least 128
-// keys a split.
 inline AttendPlan attend_plan(int n_rows, int n_seqs, int n_heads, int n_kv_heads, int head_dim, int prefix_len,
                               int max_len, bool ragged, int cus) {
   AttendPlan p{};
   const int64_t g = n_heads / n_kv_heads, cols = n_rows * g;
-  const int64_t want = 4 * (int64_t)cus;
-  auto split = [&](int64_t units, int64_t keys, int *splits, int *chunk) {
+  const int64_t want = 3 * (int64_t)cus;
+  // a block's four waves go to columns as far as there are some, the rest to keys
+  auto waves = [](int64_t c) { return c > 32 ? 4 : c > 16 ? 2 : 1; };
+  auto split = [&](int64_t units, int64_t keys, int w, int *splits, int *chunk) {
+    const int64_t step = AT_KEYS * (AT_WAVES / w);  // keys of a block's step
     int64_t n = at_ceil(want, units > 0 ? units : 1);
-    const int64_t most = at_ceil(keys, 128);
+    const int64_t most = at_ceil(keys, 2 * step);
     n = n > most ? most : n;
     n = n < 1 ? 1 : n;
-    const int64_t c = at_ceil(at_ceil(keys, n), AT_KEYS) * AT_KEYS;
+    const int64_t c = at_ceil(at_ceil(keys, n), step) * step;
     *chunk = (int)c;
     *splits = (int)at_ceil(keys, c);
   };
-  if (prefix_len > 0) {
-    p.pre_tiles = (int)at_ceil(cols, AT_COLS);
-    split((int64_t)p.pre_tiles * n_kv_heads, prefix_len, &p.pre_splits, &p.pre_chunk);
+  p.fused = prefix_len > 0 && max_len > 0 && (int64_t)prefix_len + max_len <= 512;
+  const int64_t before = p.fused ? at_ceil(prefix_len, AT_KEYS) * AT_KEYS : 0;
+  p.pre_waves = waves(cols);
+  if (prefix_len > 0 && !p.fused) {
+    p.pre_tiles = (int)at_ceil(cols, AT_COLS * p.pre_waves);
+    split((int64_t)p.pre_tiles * n_kv_heads, prefix_len, p.pre_waves, &p.pre_splits, &p.pre_chunk);
   }
+  p.own_waves = waves(ragged ? cols / (n_seqs > 0 ? n_seqs : 1) : g);
   if (max_len > 0) {
-    // sequence s's tiles start at slot floor(row_start[s] g / 16) + s
-    p.own_slots = (int)(ragged ? cols / AT_COLS + n_seqs : n_seqs * at_ceil(g, AT_COLS));
-    split((int64_t)p.own_slots * n_kv_heads, max_len, &p.own_splits, &p.own_chunk);
+    // sequence s's tiles start at slot floor(row_start[s] g / columns) + s
+    const int64_t c = AT_COLS * p.own_waves;
+    p.own_slots = (int)(ragged ? cols / c + n_seqs : n_seqs * at_ceil(g, c));
+    if (p.fused) {
+      p.own_splits = 1;
+      p.own_chunk = (int)(before + at_ceil(max_len, AT_KEYS) * AT_KEYS);
+    } else {
+      split((int64_t)p.own_slots * n_kv_heads, max_len, p.own_waves, &p.own_splits, &p.own_chunk);
+    }
   }
-  const int64_t slots = p.pre_splits + p.own_splits, items = slots * n_rows * n_heads;
+  const int64_t items = p.direct() ? 0 : (int64_t)p.slots() * n_rows * n_heads;
   p.ml_at = (size_t)items * head_dim * 4;
   p.bytes = p.ml_at + (size_t)items * 8;
   p.blocks = ((int64_t)p.pre_tiles * p.pre_splits + (int64_t)p.own_slots * p.own_splits) * n_kv_heads;
@@ -305,6 +321,11 @@ struct At8<float> {
 
 // 2^x to 1 ulp; results below the normal range are 0
 __device__ __forceinline__ float at_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// the logarithm of a sum l in units of 2^m (no key: -inf; NaN stays)
+__device__ __forceinline__ float at_lse(float m, float l) {
+  return l == 0 ? -INFINITY : m == -INFINITY ? l : (m + log2f(l)) * 0.6931471805599453f;
+}
 
 // the first row of sequence s, inside the rows there are
 __device__ __forceinline__ int at_row(const int *row_start, int s, int n_rows) {
@@ -448,210 +469,291 @@ struct AtWave {
   }
 };
 
-// whether an element of a value lane is not finite
+// whether a word of values holds one that is not finite
 template <typename CT>
 __device__ __forceinline__ bool at_odd(uint32_t w) {
-  if (sizeof(CT) == 4) return (w & 0x7f800000u) == 0x7f800000u;
-  constexpr uint32_t e = __is_same(CT, __bf16) ? 0x7f80u : 0x7c00u;
-  return (w & e) == e || ((w >> 16) & e) == e;
+  if constexpr (sizeof(CT) == 4) {
+    return (w & 0x7f800000u) == 0x7f800000u;
+  } else {
+    constexpr uint32_t e = __is_same(CT, __bf16) ? 0x7f80u : 0x7c00u;
+    return ((w & e) == e) | ((w >> 16 & e) == e);
+  }
 }
 
+// a word of values with 0 in place of what is not finite
+template <typename CT>
+__device__ __forceinline__ uint32_t at_finite(uint32_t w) {
+  if constexpr (sizeof(CT) == 4) return at_odd<CT>(w) ? 0 : w;
+  return (at_odd<CT>(w & 0xffffu) ? 0 : w & 0xffffu) | (at_odd<CT>(w & 0xffff0000u) ? 0 : w & 0xffff0000u);
+}
+
+// 2 waves on a SIMD for f32 caches, whose tiles take twice the registers, else 3
 template <typename RT, typename CT, int HD>
-__global__ __launch_bounds__(64 * AT_WAVES) void paged_attend_kernel(AttendArgs a) {
+__global__ __launch_bounds__(64 * AT_WAVES, sizeof(CT) == 4 && HD == 128 ? 2 : 3) void paged_attend_kernel(AttendArgs a) {
   using Y = AtTypes<RT, CT, HD>;
   constexpr int VW = Y::F32 ? Y::VE : Y::VE / 2;  // 32-bit words of a value lane's key
-  __shared__ float so[AT_WAVES][Y::VE][64 * 4];
-  __shared__ float sm[AT_WAVES][AT_COLS], sl[AT_WAVES][AT_COLS];
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int lane = tid & 63, g = lane >> 4, c = lane & 15;
+  __shared__ f32x4 so[AT_WAVES - 1][Y::VE][64];
+  __shared__ float sm[AT_WAVES - 1][64], sl[AT_WAVES - 1][64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int hkv = a.kv.n_kv_heads, kvh = blockIdx.x % hkv;
   int b = blockIdx.x / hkv, slot;
 
-  // the block's keys [k0, k1) by page ids, and its column: row, head, keys seen
-  const int *ids;
-  int n_ids, k0, k1, row = -1, seen = 0;
-  const int head = kvh * a.group;
-  int col;
+  // The block's keys are a run [k0, k1) of one or two page lists laid end to
+  // end: the prefix up to `pre` (rounded up to a step), then the sequence's
+  // own up to `end`.  A wave has 16 columns: row, query head, own keys seen.
+  const int *ids = nullptr;
+  int pre = 0, end = 0, k0, k1, row = -1, seen = 0, waves, col, last_seen = 0;
   if (b < a.pre_tiles * a.pre_splits) {
     slot = b / a.pre_tiles;
-    col = (b - slot * a.pre_tiles) * AT_COLS + c;
-    const int rows = a.row_start ? at_row(a.row_start, a.n_seqs, a.n_rows) : a.n_rows;
-    if (col - c >= rows * a.group) return;
+    waves = a.pre_waves;
+    const int tile = b - slot * a.pre_tiles, rows = a.row_start ? at_row(a.row_start, a.n_seqs, a.n_rows) : a.n_rows;
+    if (tile * waves * AT_COLS >= rows * a.group) return;
+    col = (tile * waves + wave % waves) * AT_COLS + c;
     if (col < rows * a.group) row = col / a.group;
-    ids = a.prefix_pages;
-    n_ids = a.prefix_count;
+    pre = a.prefix_len;
     k0 = slot * a.pre_chunk;
-    k1 = min(a.prefix_len, k0 + a.pre_chunk);
-    seen = k1;
+    k1 = min(pre, k0 + a.pre_chunk);
   } else {
     b -= a.pre_tiles * a.pre_splits;
     slot = b / a.own_slots;
     b -= slot * a.own_slots;
+    waves = a.own_waves;
+    const int tc = waves * AT_COLS;
     int s, tile, r0, r1;
     if (a.row_start) {
-      s = at_search(a.n_seqs, b, [&](int i) { return at_row(a.row_start, i, a.n_rows) * a.group / AT_COLS + i; });
+      s = at_search(a.n_seqs, b, [&](int i) { return at_row(a.row_start, i, a.n_rows) * a.group / tc + i; });
       if (s < 0) return;
       r0 = at_row(a.row_start, s, a.n_rows);
       r1 = at_row(a.row_start, s + 1, a.n_rows);
-      tile = b - (r0 * a.group / AT_COLS + s);
+      tile = b - (r0 * a.group / tc + s);
     } else {
-      const int tiles = (a.group + AT_COLS - 1) / AT_COLS;
+      const int tiles = (a.group + tc - 1) / tc;
       s = b / tiles;
       tile = b - s * tiles;
       r0 = s;
       r1 = s + 1;
     }
-    col = tile * AT_COLS + c;
     const int cols = (r1 - r0) * a.group;
-    if (col - c >= cols) return;
-    const int j = min(col, cols - 1) / a.group;
-    // the last column of the tile sees the most
-    const int last = min(col - c + AT_COLS, cols) - 1, len = min(max(a.lens[s], 0), a.max_len + (r1 - r0));
-    seen = min(len - (r1 - r0 - 1 - j), a.max_len);
+    if (tile * tc >= cols) return;
+    col = tile * tc + wave % waves * AT_COLS + c;
+    // the j-th of n rows sees len - (n - 1 - j) keys
+    const int len = min(max(a.lens[s], 0), a.max_len + (r1 - r0)) - (r1 - r0 - 1);
+    auto sees = [&](int x) { return max(min(len + x / a.group, a.max_len), 0); };
+    last_seen = sees(min(tile * tc + tc, cols) - 1);
+    seen = sees(min(col, cols - 1));
+    if (col < cols) row = r0 + col / a.group;
+    pre = a.fused ? a.prefix_len : 0;
+    end = last_seen;
+    const int before = (pre + AT_KEYS - 1) & -AT_KEYS;
     k0 = slot * a.own_chunk;
-    k1 = min(min(len - (r1 - r0 - 1 - last / a.group), a.max_len), k0 + a.own_chunk);
-    if (k1 <= k0) return;
-    seen = min(seen, k1);
-    if (col < cols) row = r0 + j;
-    else seen = k1;
-    ids = a.table + (int64_t)s * a.table_stride;
-    n_ids = a.table_width;
+    k1 = min(before + end, k0 + a.own_chunk);
     slot += a.pre_splits;
+    const bool direct = a.pre_splits + a.own_splits == 1;
+    if (k1 <= k0 && !direct) return;
+    ids = a.table + (int64_t)s * a.table_stride;
   }
-  const int hq = row >= 0 ? head + (col - col / a.group * a.group) : 0;
+  const int before = (pre + AT_KEYS - 1) & -AT_KEYS;
+  const int head = kvh * a.group + (row >= 0 ? col % a.group : 0);
 
   AtWave<RT, CT, HD> w;
-  w.init(row >= 0 ? (const RT *)a.q + row * a.q_row + hq * a.q_head : nullptr, a.scale);
+  w.init(row >= 0 ? (const RT *)a.q + row * a.q_row + head * a.q_head : nullptr, a.scale);
 
-  // what the column that sees least sees: keys before it need no mask
-  int least = seen;
+  // what the wave's column that sees least sees: keys before it need no mask
+  int least = row >= 0 ? seen : last_seen;
   least = min(least, __shfl_xor(least, 1, 64));
   least = min(least, __shfl_xor(least, 2, 64));
   least = min(least, __shfl_xor(least, 4, 64));
   least = min(least, __shfl_xor(least, 8, 64));
+  least = __builtin_amdgcn_readfirstlane(least);
 
-  const CT *kb = (const CT *)a.kv.k + kvh * a.kv.head_stride, *vb = (const CT *)a.kv.v + kvh * a.kv.head_stride;
-  const int64_t ts = a.kv.token_stride;
-  const int64_t k_lane = c * ts + (Y::F32 ? 4 * g : 8 * g), v_lane = 4 * g * ts + Y::VE * c;
+  // uniform base addresses, and 32-bit offsets of a lane in a tile of 16 keys
+  const char *kb = (const char *)a.kv.k + kvh * a.kv.head_stride * (int64_t)sizeof(CT);
+  const char *vb = (const char *)a.kv.v + kvh * a.kv.head_stride * (int64_t)sizeof(CT);
+  const int ts = (int)a.kv.token_stride * (int)sizeof(CT);
+  const uint32_t k_lane = c * ts + 16 * g, v_lane = 4 * g * ts + Y::VE * c * (int)sizeof(CT);
+  const int key_waves = AT_WAVES / waves, key_wave = wave / waves;
+  const int stride = AT_KEYS * key_waves;
+
+  u32x4 k[2][Y::KC];
+  uint32_t v[8][VW];
   for (int base = k0; base < k1; base += 1024) {
-    // lane i holds the page of keys base + 16 i ..
-    const int my_page = base + 16 * lane < k1 ? pg_page(ids, n_ids, base + 16 * lane, a.kv.page_shift, a.kv.n_pages) : -1;
-    for (int t = wave; t < 32 && base + AT_KEYS * t < k1; t += AT_WAVES) {
-      const int key0 = base + AT_KEYS * t;
-      u32x4 k[2][Y::KC];
-      uint32_t v[8][VW];
-      bool whole = least >= key0 + AT_KEYS, there[2];
+    // lane i finds the tile of keys base + 16 i .. (bytes from the pools'
+    // starts); an absent tile reads the first page, and none of it is seen
+    const int stop = min(k1, base + 1024);
+    int page = -1, slot_in = 0;
+    {
+      const int x = base + 16 * lane;
+      if (x < before) {
+        slot_in = x;
+        if (x < pre) page = pg_page(a.prefix_pages, a.prefix_count, x, a.kv.page_shift, a.kv.n_pages);
+      } else if (x < stop) {
+        slot_in = x - before;
+        page = pg_page(ids, a.table_width, slot_in, a.kv.page_shift, a.kv.n_pages);
+      }
+    }
+    const uint64_t have = __ballot(page >= 0);
+    const int64_t my_at = page < 0 ? 0 : page * a.kv.page_stride * (int64_t)sizeof(CT) + (int64_t)(slot_in & (a.kv.page_size - 1)) * ts;
+    const int at_lo = (int)my_at, at_hi = (int)(my_at >> 32);
+    auto place = [&](int x, int h) -> int64_t {
+      const int i = ((x - base) >> 4) + h;
+      return (int64_t)__builtin_amdgcn_readlane(at_hi, i) << 32 | (uint32_t)__builtin_amdgcn_readlane(at_lo, i);
+    };
+    auto load_k = [&](int x) {
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const int page = __builtin_amdgcn_readlane(my_page, 2 * t + h);
-        there[h] = page >= 0;
-        whole = whole && there[h];
-        // an absent tile reads the pool's first page, and sees none of it
-        const int64_t at = there[h] ? page * a.kv.page_stride + ((key0 + 16 * h) & (a.kv.page_size - 1)) * ts : 0;
+        const char *p = kb + place(x, h);
 #pragma unroll
-        for (int j = 0; j < Y::KC; j++) k[h][j] = *(const u32x4 *)(kb + at + k_lane + (Y::F32 ? 16 : 32) * j);
+        for (int j = 0; j < Y::KC; j++) k[h][j] = *(const u32x4 *)(p + k_lane + 64 * j);
+      }
+    };
+    auto load_v = [&](int x) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const CT *p = vb + at + v_lane + i * ts;
+      for (int h = 0; h < 2; h++) {
+        const char *p = vb + place(x, h);
+#pragma unroll
+        for (int i = 0; i < 4; i++, p += ts) {
           if constexpr (VW == 2) {
-            const u32x2 x = *(const u32x2 *)p;
-            v[4 * h + i][0] = x[0];
-            v[4 * h + i][1] = x[1];
+            const u32x2 y = *(const u32x2 *)(p + v_lane);
+            v[4 * h + i][0] = y[0];
+            v[4 * h + i][1] = y[1];
           } else {
 #pragma unroll
-            for (int y = 0; y < VW; y += 4) {
-              const u32x4 x = *(const u32x4 *)(p + y * 4 / sizeof(CT));
+            for (int z = 0; z < VW; z += 4) {
+              const u32x4 y = *(const u32x4 *)(p + v_lane + 4 * z);
 #pragma unroll
-              for (int z = 0; z < 4; z++) v[4 * h + i][y + z] = x[z];
+              for (int u = 0; u < 4; u++) v[4 * h + i][z + u] = y[u];
             }
           }
         }
       }
-      float x[8];
+    };
+    int x = base + AT_KEYS * key_wave;
+    if (x >= stop) continue;
+    load_k(x);
+    load_v(x);
+    // The next step's keys are asked for when this one's scores are taken, its
+    // values when this one's are summed: one of the two is always on its way.
+    // The last step asks for itself again, so that the number of loads in
+    // flight is the same on every path and the waits can be exact.
+    for (;;) {
+      const int next = x + stride < stop ? x + stride : x;
+      float p[8];
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         const f32x4 s = w.score(k[h]);
 #pragma unroll
-        for (int i = 0; i < 4; i++) x[4 * h + i] = s[i] * w.qs;
+        for (int i = 0; i < 4; i++) p[4 * h + i] = s[i] * w.qs;
       }
-      bool odd = false;
-      if (!whole) {
+      load_k(next);
+      const uint32_t there = (uint32_t)(have >> ((x - base) >> 4)) & 3;
+      // keys of this list that are seen: by the column, by all, by any
+      const bool shared = x < before;
+      const int x0 = shared ? x : x - before;
+      const int lim = shared ? pre : seen, all = shared ? pre : least, any = shared ? pre : end;
+      uint32_t odd = 0;  // bit j: the lane's part of key j is not finite, and not seen by all
+      if (all < x0 + AT_KEYS || there != 3) {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-          const int key = key0 + 16 * (j >> 2) + 4 * g + (j & 3);
-          if (key >= seen || !there[j >> 2]) x[j] = -INFINITY;
+          const int key = x0 + 16 * (j >> 2) + 4 * g + (j & 3);
+          const bool is = there >> (j >> 2) & 1;
+          p[j] = is & (key < lim) ? p[j] : -INFINITY;
           // a value that no column sees may be anything, and 0 times it not 0
-          const bool none = key >= k1 || !there[j >> 2];
+          const bool none = !is | (key >= any);
+          bool bad = false;
 #pragma unroll
           for (int y = 0; y < VW; y++) {
-            if (none) v[j][y] = 0;
-            odd = odd || (key >= least && at_odd<CT>(v[j][y]));
+            v[j][y] = none ? 0 : v[j][y];
+            bad |= at_odd<CT>(v[j][y]);
+          }
+          odd |= (uint32_t)(bad & (key >= all)) << j;
+        }
+      }
+      w.softmax(p);
+      if (__any(odd)) {
+        // such elements are taken out of the common product and added to the
+        // columns that see them one by one, each lane to its own dimensions
+        for (int j = 0; j < 8; j++) {
+          const uint64_t lanes = __ballot(odd >> j & 1);
+#pragma unroll
+          for (int jj = 0; jj < 8; jj++)
+#pragma unroll
+            for (int y = 0; y < VW; y++) v[jj][y] = jj == j && (odd >> j & 1) ? at_finite<CT>(v[jj][y]) : v[jj][y];
+          float pj = p[0];
+#pragma unroll
+          for (int jj = 1; jj < 8; jj++) pj = jj == j ? p[jj] : pj;
+          for (int gg = 0; gg < 4; gg++) {
+            if (!(lanes >> (16 * gg) & 0xffff)) continue;
+            const int in = 4 * gg + (j & 3);
+            const float weight = __shfl(pj, 16 * gg + c, 64);
+            const CT *row = (const CT *)(vb + place(x, j >> 2) + (int64_t)in * ts) + 4 * Y::VE * g;
+            if (x0 + 16 * (j >> 2) + in < lim) {
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                float y[Y::VE];
+                pg_load(row + Y::VE * i, y);
+#pragma unroll
+                for (int e = 0; e < Y::VE; e++)
+                  if (!(fabsf(y[e]) < INFINITY)) w.o[e][i] = fmaf(weight, y[e], w.o[e][i]);
+              }
+            }
           }
         }
       }
-      w.softmax(x);
-      if (!__any(odd)) {
-        w.values(x, v);
-      } else {
-        // A value that only some columns see is not finite: one column at a
-        // time, with the values it does not see put to zero.
-        for (int cc = 0; cc < AT_COLS; cc++) {
-          const int lim = __builtin_amdgcn_readlane(seen, cc);
-          uint32_t u[8][VW];
-          f32x4 keep[Y::VE];
-#pragma unroll
-          for (int j = 0; j < 8; j++)
-#pragma unroll
-            for (int y = 0; y < VW; y++)
-              u[j][y] = key0 + 16 * (j >> 2) + 4 * g + (j & 3) < lim ? v[j][y] : 0;
-#pragma unroll
-          for (int e = 0; e < Y::VE; e++) keep[e] = w.o[e];
-          w.values(x, u);
-#pragma unroll
-          for (int e = 0; e < Y::VE; e++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) w.o[e][i] = c == cc ? w.o[e][i] : keep[e][i];
-        }
-      }
+      w.values(p, v);
+      load_v(next);
+      if (next == x) break;
+      x = next;
     }
   }
 
-  // join the waves' states: each scaled to the common maximum
+  // the waves with the same columns join their states in the first one's
   w.l = at_sum4(w.l);
-  if (g == 0) {
-    sm[wave][c] = w.m;
-    sl[wave][c] = w.l;
+  if (key_waves > 1) {
+    if (key_wave > 0) {
+      const int at = wave - waves;
+#pragma unroll
+      for (int e = 0; e < Y::VE; e++) so[at][e][lane] = w.o[e];
+      sm[at][lane] = w.m;
+      sl[at][lane] = w.l;
+    }
+    __syncthreads();
+    if (key_wave > 0) return;
+    for (int i = 1; i < key_waves; i++) {
+      const int at = wave + (i - 1) * waves;
+      const float m1 = sm[at][lane], m = fmaxf(w.m, m1);
+      // (a state without a maximum holds zeros, or NaN, which must not get lost)
+      const float f0 = w.m == -INFINITY ? 1.0f : at_exp2(w.m - m), f1 = m1 == -INFINITY ? 1.0f : at_exp2(m1 - m);
+      w.m = m;
+      w.l = w.l * f0 + sl[at][lane] * f1;
+#pragma unroll
+      for (int e = 0; e < Y::VE; e++) w.o[e] = w.o[e] * f0 + so[at][e][lane] * f1;
+    }
   }
-  __syncthreads();
-  float m = sm[0][c];
+  if (row < 0) return;
+  // the lane's dimensions: 4 VE from 4 VE g on
+  if (a.pre_splits + a.own_splits == 1) {
+    const float r = w.l == 0 ? 0.0f : 1.0f / w.l;
+    RT *out = (RT *)a.out + row * a.o_row + head * a.o_head + 4 * Y::VE * g;
 #pragma unroll
-  for (int i = 1; i < AT_WAVES; i++) m = fmaxf(m, sm[i][c]);
-  // (a state without a maximum holds zeros, or NaN, which must not get lost)
-  const float f = w.m == -INFINITY ? 1.0f : at_exp2(w.m - m);
+    for (int i = 0; i < 4; i++) {
+      float y[Y::VE];
 #pragma unroll
-  for (int e = 0; e < Y::VE; e++) *(f32x4 *)&so[wave][e][lane * 4] = w.o[e] * f;
-  __syncthreads();
-  // thread (lane ln, i): dimensions VE (4 (ln >> 4) + i) .. of column ln & 15
-  const int ln = tid >> 2, i = tid & 3, cc = ln & 15;
-  const int row2 = __shfl(row, cc, 64), hq2 = __shfl(hq, cc, 64);
-  if (row2 < 0) return;
-  float y[Y::VE];
-#pragma unroll
-  for (int e = 0; e < Y::VE; e++) {
-    y[e] = so[0][e][tid];
-#pragma unroll
-    for (int u = 1; u < AT_WAVES; u++) y[e] += so[u][e][tid];
+      for (int e = 0; e < Y::VE; e++) y[e] = w.o[e][i] * r;
+      pg_store(out + Y::VE * i, y);
+    }
+    if (a.lse && g == 0) a.lse[(int64_t)row * a.n_heads + head] = at_lse(w.m, w.l);
+    return;
   }
-  const int64_t item = ((int64_t)slot * a.n_rows + row2) * a.n_heads + hq2;
-  pg_store(a.part_o + item * HD + Y::VE * (4 * (ln >> 4) + i), y);
-  if (ln < AT_COLS && i == 0) {
-    float mm = sm[0][cc], l = 0;
+  const int64_t item = ((int64_t)slot * a.n_rows + row) * a.n_heads + head;
 #pragma unroll
-    for (int u = 1; u < AT_WAVES; u++) mm = fmaxf(mm, sm[u][cc]);
+  for (int i = 0; i < 4; i++) {
+    float y[Y::VE];
 #pragma unroll
-    for (int u = 0; u < AT_WAVES; u++) l += sl[u][cc] * (sm[u][cc] == -INFINITY ? 1.0f : at_exp2(sm[u][cc] - mm));
-    a.part_ml[item] = make_float2(mm, l);
+    for (int e = 0; e < Y::VE; e++) y[e] = w.o[e][i];
+    pg_store(a.part_o + item * HD + 4 * Y::VE * g + Y::VE * i, y);
   }
+  if (g == 0) a.part_ml[item] = make_float2(w.m, w.l);
 }
 
 // Joins a row and head's partials, a wave each: lane l takes dimensions
@@ -693,7 +795,7 @@ __global__ __launch_bounds__(256) void paged_attend_join_kernel(AttendArgs a) {
 #pragma unroll
   for (int j = 0; j < N; j++) y[j] *= r;
   pg_store((RT *)a.out + row * a.o_row + head * a.o_head + N * lane, y);
-  if (a.lse && lane == 0) a.lse[item] = l == 0 ? -INFINITY : (m == -INFINITY ? l : (m + log2f(l)) * 0.6931471805599453f);
+  if (a.lse && lane == 0) a.lse[item] = at_lse(m, l);
 }
 
 }  // namespace vx
