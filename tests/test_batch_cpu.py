@@ -155,19 +155,20 @@ int main() {
       for (int len : lens)
         for (int pre : lens)
           for (int hd : {64, 128})
-            for (bool ragged : {false, true}) {
+            for (bool ragged : {false, true})
+            for (int wide_cols : {0, 64, 128}) {
               const int seqs = ragged ? (r + 2) / 3 : r, g = h[0] / h[1];
-              const AttendPlan p = attend_plan(r, seqs, h[0], h[1], hd, pre, len, ragged, 256);
+              const AttendPlan p = attend_plan(r, seqs, h[0], h[1], hd, pre, len, ragged, wide_cols, 256);
               if (pre && !p.fused && ((int64_t)p.pre_splits * p.pre_chunk < pre || (int64_t)(p.pre_splits - 1) * p.pre_chunk >= pre ||
-                                      p.pre_chunk % 32 || (int64_t)p.pre_tiles * AT_COLS * p.pre_waves < (int64_t)r * g))
+                                      p.pre_chunk % 32 || (int64_t)p.pre_tiles * p.pre_cols < (int64_t)r * g))
                 return 3;
               // a fused block's keys: the prefix in whole steps, then its own
               const int64_t own = len + (p.fused ? at_ceil(pre, 32) * 32 : 0);
               if (len && ((int64_t)p.own_splits * p.own_chunk < own || (int64_t)(p.own_splits - 1) * p.own_chunk >= own || p.own_chunk % 32))
                 return 4;
               if (p.fused && (p.pre_splits || p.pre_tiles || !len)) return 5;
-              for (int w : {p.pre_waves, p.own_waves})
-                if (w != 1 && w != 2 && w != 4) return 9;
+              if (p.pre_wide ? p.pre_cols != wide_cols : p.pre_cols != 16 && p.pre_cols != 32 && p.pre_cols != 64) return 9;
+              if (p.own_wide ? p.own_cols != wide_cols : p.own_cols != 16 && p.own_cols != 32 && p.own_cols != 64) return 9;
               if (p.blocks > 0x7fffffff || p.ml_at % 16) return 6;
               const size_t items = (size_t)(p.pre_splits + p.own_splits) * r * h[0];
               if (!p.direct() && (p.bytes < items * (hd * 4 + 8) || p.ml_at < items * hd * 4)) return 7;
@@ -178,7 +179,7 @@ int main() {
               for (int s = 0; s < seqs; s++) {
                 const int n = !ragged ? 1 : s + 1 < seqs ? (s * 7) % 4 : r - r0;
                 const int r1 = r0 + n < r ? r0 + n : r;
-                const int tc = AT_COLS * p.own_waves, tiles = (int)at_ceil((int64_t)(r1 - r0) * g, tc);
+                const int tc = p.own_cols, tiles = (int)at_ceil((int64_t)(r1 - r0) * g, tc);
                 const int64_t first = ragged ? (int64_t)r0 * g / tc + s : (int64_t)s * at_ceil(g, tc);
                 for (int t = 0; t < tiles; t++)
                   if (first + t >= p.own_slots || taken[first + t]++) return 8;

@@ -160,7 +160,7 @@ inline int check_attend(const char *what, const vx_attend_args *p, PagedKV *kv, 
   if (!p->row_start && p->n_seqs != p->n_rows)
     return batch_fail(VX_E_INVALID, "%s: %d rows of %d sequences without row_start", what, p->n_rows, p->n_seqs);
   *plan = attend_plan(p->n_rows, p->n_seqs, p->n_heads, p->kv.n_kv_heads, p->kv.head_dim, p->prefix_len, p->max_len,
-                      p->row_start != nullptr, device_cus(p->kv.device));
+                      p->row_start != nullptr, at_wide_cols(type_size(p->type), type_size(p->kv.type)), device_cus(p->kv.device));
   return VX_OK;
 }
 
@@ -184,9 +184,11 @@ inline int paged_attend(const vx_attend_args *p, void *stream) {
   a.prefix_len = p->prefix_len, a.max_len = p->max_len;
   a.n_rows = p->n_rows, a.n_seqs = p->n_seqs, a.n_heads = p->n_heads, a.group = p->n_heads / p->kv.n_kv_heads;
   a.scale = (p->scale == 0 ? 1.0f / sqrtf((float)p->kv.head_dim) : p->scale) * 1.4426950408889634f;
-  a.pre_waves = plan.pre_waves, a.pre_tiles = plan.pre_tiles, a.pre_splits = plan.pre_splits, a.pre_chunk = plan.pre_chunk;
-  a.own_waves = plan.own_waves, a.own_slots = plan.own_slots, a.own_splits = plan.own_splits, a.own_chunk = plan.own_chunk;
-  a.fused = plan.fused;
+  a.pre_cols = plan.pre_cols, a.pre_wide = plan.pre_wide, a.pre_tiles = plan.pre_tiles;
+  a.pre_splits = plan.pre_splits, a.pre_chunk = plan.pre_chunk;
+  a.own_cols = plan.own_cols, a.own_wide = plan.own_wide, a.own_slots = plan.own_slots;
+  a.own_splits = plan.own_splits, a.own_chunk = plan.own_chunk;
+  a.fused = plan.fused, a.team = plan.team;
   a.part_o = (float *)p->workspace;
   a.part_ml = (float2 *)((char *)p->workspace + plan.ml_at);
   OnDevice on(p->kv.device);
@@ -194,12 +196,18 @@ inline int paged_attend(const vx_attend_args *p, void *stream) {
   return with_types(p->type, p->kv.type, [&](auto r, auto c) {
     auto go = [&](auto part, auto join) {
       int rc = plan.blocks ? batch_launch(what, part, plan.blocks, 64 * AT_WAVES, 0, a, stream) : VX_OK;
-      return rc || plan.direct() ? rc : batch_launch(what, join, at_ceil((int64_t)a.n_rows * a.n_heads, 4), 256, 0, a, stream);
+      return rc || plan.direct() ? rc : batch_launch(what, join, at_ceil((int64_t)a.n_rows * a.n_heads, AT_WAVES / a.team), 64 * AT_WAVES, 0, a, stream);
     };
     using R = decltype(r);
     using C = decltype(c);
-    return p->kv.head_dim == 128 ? go(paged_attend_kernel<R, C, 128>, paged_attend_join_kernel<R, 128>)
-                                 : go(paged_attend_kernel<R, C, 64>, paged_attend_join_kernel<R, 64>);
+    const bool hd128 = p->kv.head_dim == 128;
+    if constexpr (AtTypes<R, C, 128>::WIDE > 0) {
+      if ((plan.pre_wide && plan.pre_splits) || plan.own_wide)
+        return hd128 ? go(paged_attend_kernel<R, C, 128, true>, paged_attend_join_kernel<R, 128>)
+                     : go(paged_attend_kernel<R, C, 64, true>, paged_attend_join_kernel<R, 64>);
+    }
+    return hd128 ? go(paged_attend_kernel<R, C, 128, false>, paged_attend_join_kernel<R, 128>)
+                 : go(paged_attend_kernel<R, C, 64, false>, paged_attend_join_kernel<R, 64>);
   });
 }
 

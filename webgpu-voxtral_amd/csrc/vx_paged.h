@@ -170,12 +170,20 @@ __global__ __launch_bounds__(PA_NT) void paged_append_kernel(AppendArgs a) {
 // Row r of sequence s, the j-th of its n_s rows: one softmax over the shared
 // prefix's keys and the first clamp(lens[s] - (n_s - 1 - j), 0, max_len) keys
 // of the sequence.  Columns: the n_s rows times the G query heads of a KV
-// head, row-major, 16 to a wave.  Blocks of the first kind take the prefix
-// with the columns of all rows, so its keys are read once for many columns
-// and not once a sequence; blocks of the second kind take a sequence's own
-// keys (and, where that is little, the prefix before them: `fused`).  Both
-// split the key axis and leave (o, m, l) partials that a second kernel joins,
-// unless there is one split in all.
+// head, row-major.  Blocks of the first kind take the prefix with the columns
+// of all rows, so its keys are read once for many columns and not once a
+// sequence; blocks of the second kind take a sequence's own keys and, where
+// `fused`, the prefix before them.  Both split the key axis and leave
+// (o, m, l) partials that a second kernel joins, unless there is one split in
+// all.
+//
+// Few columns (a decode step's own keys): the block's four waves go to
+// different columns, 16 each, or share columns and split the keys; a wave
+// brings its keys and values from memory to registers by itself.  That is
+// bound by HBM: the matrix cores are all but idle.  Many columns (wide): the
+// waves bring 128 keys together through LDS, laid out as the matrix
+// instruction's operands, and each takes 32 columns (16 for f32 rows) through
+// all of them.
 struct AttendArgs {
   PagedKV kv;
   const void *q;
@@ -187,21 +195,22 @@ struct AttendArgs {
   int table_width, prefix_count, prefix_len, max_len;
   int n_rows, n_seqs, n_heads, group;
   float scale;  // times log2(e)
-  // the plan: column waves of a block, tiles of columns, splits and their
-  // keys (multiples of 32)
-  int pre_waves, pre_tiles, pre_splits, pre_chunk;
-  int own_waves, own_slots, own_splits, own_chunk;
-  int fused;
-  float *part_o;   // [slot][row * heads + head][head_dim]
+  // the plan: columns of a block (over 64: wide), tiles of columns, splits and
+  // their keys (multiples of 32)
+  int pre_cols, pre_wide, pre_tiles, pre_splits, pre_chunk;
+  int own_cols, own_wide, own_slots, own_splits, own_chunk;
+  int fused, team;
+  float *part_o;   // [slot][row * heads + head][e][r]: dimension VE r + e
   float2 *part_ml; // [slot][row * heads + head]: maximum (log2 units), sum
 };
 
-constexpr int AT_COLS = 16;  // columns of a wave: the matrix instruction's
-constexpr int AT_KEYS = 32;  // keys of a wave's step: two tiles of 16
+constexpr int AT_COLS = 16;  // columns of a matrix instruction
+constexpr int AT_KEYS = 32;  // prefixes and splits are cut in multiples of this
 constexpr int AT_WAVES = 4;
+constexpr int AT_STAGE = AT_KEYS * AT_WAVES;  // keys that a wide block brings at a time
 
 struct AttendPlan {
-  int pre_waves, pre_tiles, pre_splits, pre_chunk, own_waves, own_slots, own_splits, own_chunk, fused;
+  int pre_cols, pre_wide, pre_tiles, pre_splits, pre_chunk, own_cols, own_wide, own_slots, own_splits, own_chunk, fused, team;
   size_t ml_at, bytes;  // the workspace: part_o, then part_ml at ml_at
   int64_t blocks;
   int slots() const { return pre_splits + own_splits; }
@@ -210,43 +219,44 @@ struct AttendPlan {
 
 __host__ __device__ inline int64_t at_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// wide_cols: columns of a wide block (0: there is none for these types)
 inline AttendPlan attend_plan(int n_rows, int n_seqs, int n_heads, int n_kv_heads, int head_dim, int prefix_len,
-                              int max_len, bool ragged, int cus) {
+                              int max_len, bool ragged, int wide_cols, int cus) {
   AttendPlan p{};
   const int64_t g = n_heads / n_kv_heads, cols = n_rows * g;
-  const int64_t want = 3 * (int64_t)cus;
-  // a block's four waves go to columns as far as there are some, the rest to keys
-  auto waves = [](int64_t c) { return c > 32 ? 4 : c > 16 ? 2 : 1; };
-  auto split = [&](int64_t units, int64_t keys, int w, int *splits, int *chunk) {
-    const int64_t step = AT_KEYS * (AT_WAVES / w);  // keys of a block's step
+  // Columns of a block that has `c` of them to choose from: a narrow block's
+  // four waves go to columns as far as there are some, the rest to keys.
+  auto choose = [&](int64_t c, int *block_cols, int *wide) {
+    *wide = wide_cols && c >= 64;
+    *block_cols = *wide ? wide_cols : AT_COLS * (c > 32 ? 4 : c > 16 ? 2 : 1);
+  };
+  auto step_of = [](int block_cols, int wide) { return wide ? AT_STAGE : AT_STAGE * AT_COLS / block_cols; };
+  // splits of `keys` for about `want` blocks
+  auto split = [&](int64_t units, int64_t keys, int64_t step, int64_t want, int *splits, int *chunk) {
     int64_t n = at_ceil(want, units > 0 ? units : 1);
-    const int64_t most = at_ceil(keys, 2 * step);
+    const int64_t most = at_ceil(keys, step);
     n = n > most ? most : n;
     n = n < 1 ? 1 : n;
     const int64_t c = at_ceil(at_ceil(keys, n), step) * step;
     *chunk = (int)c;
     *splits = (int)at_ceil(keys, c);
   };
-  p.fused = prefix_len > 0 && max_len > 0 && (int64_t)prefix_len + max_len <= 512;
-  const int64_t before = p.fused ? at_ceil(prefix_len, AT_KEYS) * AT_KEYS : 0;
-  p.pre_waves = waves(cols);
+  choose(cols, &p.pre_cols, &p.pre_wide);
+  choose(ragged ? cols / (n_seqs > 0 ? n_seqs : 1) : g, &p.own_cols, &p.own_wide);
+  p.fused = prefix_len > 0 && max_len > 0 && (p.own_wide || (int64_t)prefix_len + max_len <= 512);
   if (prefix_len > 0 && !p.fused) {
-    p.pre_tiles = (int)at_ceil(cols, AT_COLS * p.pre_waves);
-    split((int64_t)p.pre_tiles * n_kv_heads, prefix_len, p.pre_waves, &p.pre_splits, &p.pre_chunk);
+    p.pre_tiles = (int)at_ceil(cols, p.pre_cols);
+    split((int64_t)p.pre_tiles * n_kv_heads, prefix_len, step_of(p.pre_cols, p.pre_wide), cus, &p.pre_splits, &p.pre_chunk);
   }
-  p.own_waves = waves(ragged ? cols / (n_seqs > 0 ? n_seqs : 1) : g);
   if (max_len > 0) {
+    const int64_t before = p.fused ? at_ceil(prefix_len, AT_KEYS) * AT_KEYS : 0;
     // sequence s's tiles start at slot floor(row_start[s] g / columns) + s
-    const int64_t c = AT_COLS * p.own_waves;
-    p.own_slots = (int)(ragged ? cols / c + n_seqs : n_seqs * at_ceil(g, c));
-    if (p.fused) {
-      p.own_splits = 1;
-      p.own_chunk = (int)(before + at_ceil(max_len, AT_KEYS) * AT_KEYS);
-    } else {
-      split((int64_t)p.own_slots * n_kv_heads, max_len, p.own_waves, &p.own_splits, &p.own_chunk);
-    }
+    p.own_slots = (int)(ragged ? cols / p.own_cols + n_seqs : n_seqs * at_ceil(g, p.own_cols));
+    split((int64_t)p.own_slots * n_kv_heads, before + max_len, step_of(p.own_cols, p.own_wide),
+          p.fused && !p.own_wide ? 1 : p.own_wide ? 2 * cus : 6 * cus, &p.own_splits, &p.own_chunk);
   }
   const int64_t items = p.direct() ? 0 : (int64_t)p.slots() * n_rows * n_heads;
+  p.team = p.slots() >= 24 ? AT_WAVES : 1;
   p.ml_at = (size_t)items * head_dim * 4;
   p.bytes = p.ml_at + (size_t)items * 8;
   p.blocks = ((int64_t)p.pre_tiles * p.pre_splits + (int64_t)p.own_slots * p.own_splits) * n_kv_heads;
@@ -294,9 +304,15 @@ template <typename RT, typename CT, int HD>
 struct AtTypes {
   static constexpr bool F32 = sizeof(CT) == 4;
   static constexpr bool SPLIT = !F32 && sizeof(RT) == 4;
-  static constexpr int VE = HD / 16;           // value instructions, dimensions a lane loads of a key
+  static constexpr int H = F32 ? 1 : 2;               // tiles of 16 keys in a wave's step
+  static constexpr int STEP = 16 * H;
+  static constexpr int VE = HD / 16;                  // value instructions, dimensions a lane loads of a key
+  static constexpr int VW = F32 ? VE : VE / 2;        // 32-bit words of a key a value lane loads
   static constexpr int KC = F32 ? HD / 16 : HD / 32;  // 16-byte chunks of a key a lane holds
+  static constexpr int WIDE = F32 ? 0 : SPLIT ? 1 : 2;  // column tiles of a wave in a wide block
 };
+// columns of a wide block by the sizes of row and cache elements
+inline int at_wide_cols(size_t row, size_t cache) { return cache == 4 ? 0 : AT_WAVES * AT_COLS * (row == 4 ? 1 : 2); }
 
 __device__ __forceinline__ f32x4 at_mma(h8 a, h8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -342,9 +358,26 @@ __device__ __forceinline__ float at_sum4(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
-// A wave's state over its keys for one tile of columns
+// whether a word of values holds one that is not finite
+template <typename CT>
+__device__ __forceinline__ bool at_odd(uint32_t w) {
+  if constexpr (sizeof(CT) == 4) {
+    return (w & 0x7f800000u) == 0x7f800000u;
+  } else {
+    constexpr uint32_t e = __is_same(CT, __bf16) ? 0x7f80u : 0x7c00u;
+    return ((w & e) == e) | ((w >> 16 & e) == e);
+  }
+}
+// a word of values with 0 in place of what is not finite
+template <typename CT>
+__device__ __forceinline__ uint32_t at_finite(uint32_t w) {
+  if constexpr (sizeof(CT) == 4) return at_odd<CT>(w) ? 0 : w;
+  return (at_odd<CT>(w & 0xffffu) ? 0 : w & 0xffffu) | (at_odd<CT>(w & 0xffff0000u) ? 0 : w & 0xffff0000u);
+}
+
+// One tile of 16 columns in a wave: queries, sums, maximum
 template <typename RT, typename CT, int HD>
-struct AtWave {
+struct AtTile {
   using Y = AtTypes<RT, CT, HD>;
   using E8 = typename At8<CT>::T;
   u32x4 q[Y::KC * (Y::SPLIT ? 2 : 1)];  // the column's queries: hi, then lo
@@ -393,65 +426,26 @@ struct AtWave {
     }
   }
 
-  // scores of 16 keys, one row of `k` (already offset to the lane's key)
-  __device__ __forceinline__ f32x4 score(const u32x4 (&k)[Y::KC]) const {
-    f32x4 s{0, 0, 0, 0};
+  // s += the products of chunk j of 16 keys
+  __device__ __forceinline__ f32x4 score(u32x4 k, int j, f32x4 s) const {
+    if constexpr (Y::F32) {
+      const f32x4 a = __builtin_bit_cast(f32x4, k), b = __builtin_bit_cast(f32x4, q[j]);
 #pragma unroll
-    for (int j = 0; j < Y::KC; j++) {
-      if constexpr (Y::F32) {
-        const f32x4 a = __builtin_bit_cast(f32x4, k[j]), b = __builtin_bit_cast(f32x4, q[j]);
-#pragma unroll
-        for (int i = 0; i < 4; i++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], s, 0, 0, 0);
-      } else {
-        s = at_mma(__builtin_bit_cast(E8, k[j]), __builtin_bit_cast(E8, q[j]), s);
-        if constexpr (Y::SPLIT) s = at_mma(__builtin_bit_cast(E8, k[j]), __builtin_bit_cast(E8, q[Y::KC + j]), s);
-      }
+      for (int i = 0; i < 4; i++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], s, 0, 0, 0);
+    } else {
+      s = at_mma(__builtin_bit_cast(E8, k), __builtin_bit_cast(E8, q[j]), s);
+      if constexpr (Y::SPLIT) s = at_mma(__builtin_bit_cast(E8, k), __builtin_bit_cast(E8, q[Y::KC + j]), s);
     }
     return s;
   }
 
-  // o += P V over 32 keys; v[j]: the lane's dimensions of key 4 g + (j & 3) of tile j >> 2
-  __device__ __forceinline__ void values(const float (&p)[8], const uint32_t (&v)[8][Y::F32 ? Y::VE : Y::VE / 2]) {
-    if constexpr (Y::F32) {
-#pragma unroll
-      for (int j = 0; j < 8; j++)
-#pragma unroll
-        for (int e = 0; e < Y::VE; e++)
-          o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, v[j][e]), p[j], o[e], 0, 0, 0);
-    } else {
-      E8 ph, pl;
-      if constexpr (Y::SPLIT) {
-        split_n(p, ph, pl);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++) ph[j] = (CT)p[j];
-      }
-#pragma unroll
-      for (int w = 0; w < Y::VE / 2; w++) {
-        u32x4 a, b;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {  // key pairs: the low halves, the high halves
-          a[j] = __builtin_amdgcn_perm(v[2 * j + 1][w], v[2 * j][w], 0x05040100u);
-          b[j] = __builtin_amdgcn_perm(v[2 * j + 1][w], v[2 * j][w], 0x07060302u);
-        }
-        const E8 va = __builtin_bit_cast(E8, a), vb = __builtin_bit_cast(E8, b);
-        o[2 * w] = at_mma(va, ph, o[2 * w]);
-        o[2 * w + 1] = at_mma(vb, ph, o[2 * w + 1]);
-        if constexpr (Y::SPLIT) {
-          o[2 * w] = at_mma(va, pl, o[2 * w]);
-          o[2 * w + 1] = at_mma(vb, pl, o[2 * w + 1]);
-        }
-      }
-    }
-  }
-
-  // the weights of 8 scores (in log2 units; -inf: not seen), with the running
+  // the weights of a step's scores (in log2 units; -inf: not seen), with the running
   // maximum moved where one passes it by more than 8: until then weights of up
   // to 2^8 do no harm, and the sums need not be scaled
-  __device__ __forceinline__ void softmax(float (&x)[8]) {
+  __device__ __forceinline__ void softmax(float (&x)[4 * Y::H]) {
     float top = x[0];
 #pragma unroll
-    for (int j = 1; j < 8; j++) top = fmaxf(top, x[j]);
+    for (int j = 1; j < 4 * Y::H; j++) top = fmaxf(top, x[j]);
     if (__any(top > m + 8.0f)) {
       const float n = fmaxf(m, at_max4(top));
       const float f = n == -INFINITY ? 1.0f : at_exp2(m - n);
@@ -462,307 +456,518 @@ struct AtWave {
     }
     const float z = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
+    for (int j = 0; j < 4 * Y::H; j++) {
       x[j] = at_exp2(x[j] - z);
       l += x[j];
     }
   }
+
+  // 16-bit caches: the weights as B operands, hi and lo
+  __device__ __forceinline__ void weights(const float (&p)[8], E8 (&b)[Y::SPLIT ? 2 : 1]) const {
+    if constexpr (Y::SPLIT) {
+      split_n(p, b[0], b[1]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) b[0][j] = (CT)p[j];
+    }
+  }
+  __device__ __forceinline__ void value(int e, u32x4 v, const E8 (&b)[Y::SPLIT ? 2 : 1]) {
+    o[e] = at_mma(__builtin_bit_cast(E8, v), b[0], o[e]);
+    if constexpr (Y::SPLIT) o[e] = at_mma(__builtin_bit_cast(E8, v), b[1], o[e]);
+  }
+
+  // Adds the elements that are not finite of a step's rows (bit r of `rows`:
+  // row r & 15 of the tile at `place(r >> 4)`) to the columns that see them, each lane
+  // to its own dimensions.  They were taken out of the common product, where
+  // 0 times them would not be 0 for the columns that do not see them.
+  template <typename F>
+  __device__ __forceinline__ void add_odd(uint32_t rows, const float (&p)[4 * Y::H], int limit, int ts, F place) {
+    const int g = (threadIdx.x & 63) >> 4, c = threadIdx.x & 15;
+    while (rows) {
+      const int r = __ffs(rows) - 1, j = 4 * (r >> 4) + (r & 3);
+      rows &= rows - 1;
+      float pj = p[0];
+#pragma unroll
+      for (int i = 1; i < 4 * Y::H; i++) pj = i == j ? p[i] : pj;
+      const float weight = __shfl(pj, (r & 12) * 4 + c, 64);
+      const CT *row = (const CT *)(place(r >> 4) + (int64_t)(r & 15) * ts) + 4 * Y::VE * g;
+      if (r < limit) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          float y[Y::VE];
+          pg_load(row + Y::VE * i, y);
+#pragma unroll
+          for (int e = 0; e < Y::VE; e++)
+            if (!(fabsf(y[e]) < INFINITY)) o[e][i] = fmaf(weight, y[e], o[e][i]);
+        }
+      }
+    }
+  }
+
+  // the column's result or partial; the lane's dimensions are 4 VE from 4 VE g on
+  __device__ __forceinline__ void store(const AttendArgs &a, int slot, int row, int head) {
+    const int g = (threadIdx.x & 63) >> 4;
+    l = at_sum4(l);
+    if (row < 0) return;
+    if (a.pre_splits + a.own_splits == 1) {
+      const float r = l == 0 ? 0.0f : 1.0f / l;
+      RT *out = (RT *)a.out + row * a.o_row + head * a.o_head + 4 * Y::VE * g;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        float y[Y::VE];
+#pragma unroll
+        for (int e = 0; e < Y::VE; e++) y[e] = o[e][i] * r;
+        pg_store(out + Y::VE * i, y);
+      }
+      if (a.lse && g == 0) a.lse[(int64_t)row * a.n_heads + head] = at_lse(m, l);
+      return;
+    }
+    const int64_t item = ((int64_t)slot * a.n_rows + row) * a.n_heads + head;
+#pragma unroll
+    for (int e = 0; e < Y::VE; e++) *(f32x4 *)(a.part_o + item * HD + 16 * e + 4 * g) = o[e];
+    if (g == 0) a.part_ml[item] = make_float2(m, l);
+  }
 };
 
-// whether a word of values holds one that is not finite
-template <typename CT>
-__device__ __forceinline__ bool at_odd(uint32_t w) {
-  if constexpr (sizeof(CT) == 4) {
-    return (w & 0x7f800000u) == 0x7f800000u;
-  } else {
-    constexpr uint32_t e = __is_same(CT, __bf16) ? 0x7f80u : 0x7c00u;
-    return ((w & e) == e) | ((w >> 16 & e) == e);
+// What a block works on.  Its keys are a run [k0, k1) of one or two page
+// lists laid end to end: the prefix up to `pre` (then up to `before`, in whole
+// steps), then a sequence's own.  Its columns are first .. first + 15 and so
+// on, those below `cols` exist; column x is row r0 + x / group.
+struct AtJob {
+  const int *ids, *prefix_ids;
+  int n_ids, n_prefix_ids;
+  int pre, before, k0, k1, slot, r0, cols, first, len, group, max_len;
+  // own keys that a column sees (it does not fall along the columns)
+  __device__ __forceinline__ int sees(int x) const { return max(min(len + min(x, cols - 1) / group, max_len), 0); }
+};
+
+// The tiles of 16 keys of a run of up to 1024: lane i holds where keys
+// base + 16 i .. lie (bytes from the pools' starts).  An absent tile points to
+// the first page, and none of it is seen.
+struct AtPages {
+  int base, at_lo, at_hi;
+  uint64_t have;
+  __device__ __forceinline__ void look(const AtJob &b, const PagedKV &kv, int from, int stop, int ts, int elem) {
+    base = from;
+    const int x = from + 16 * (threadIdx.x & 63);
+    int page = -1, slot = 0;
+    if (x < b.before) {
+      slot = x;
+      if (x < b.pre) page = pg_page(b.prefix_ids, b.n_prefix_ids, x, kv.page_shift, kv.n_pages);
+    } else if (x < stop) {
+      slot = x - b.before;
+      page = pg_page(b.ids, b.n_ids, slot, kv.page_shift, kv.n_pages);
+    }
+    have = __ballot(page >= 0);
+    const int64_t at = page < 0 ? 0 : page * kv.page_stride * elem + (int64_t)(slot & (kv.page_size - 1)) * ts;
+    at_lo = (int)at;
+    at_hi = (int)(at >> 32);
   }
-}
+  // tile h of the step at x
+  __device__ __forceinline__ int64_t place(int x, int h) const {
+    const int i = ((x - base) >> 4) + h;
+    return (int64_t)__builtin_amdgcn_readlane(at_hi, i) << 32 | (uint32_t)__builtin_amdgcn_readlane(at_lo, i);
+  }
+  // which tiles of a step of h are there, as bits
+  __device__ __forceinline__ uint32_t there(int x, int h) const { return (uint32_t)(have >> ((x - base) >> 4)) & ((1u << h) - 1); }
+};
 
-// a word of values with 0 in place of what is not finite
-template <typename CT>
-__device__ __forceinline__ uint32_t at_finite(uint32_t w) {
-  if constexpr (sizeof(CT) == 4) return at_odd<CT>(w) ? 0 : w;
-  return (at_odd<CT>(w & 0xffffu) ? 0 : w & 0xffffu) | (at_odd<CT>(w & 0xffff0000u) ? 0 : w & 0xffff0000u);
-}
-
-// 2 waves on a SIMD for f32 caches, whose tiles take twice the registers, else 3
+// A wave's registers for the keys and values of one step
 template <typename RT, typename CT, int HD>
-__global__ __launch_bounds__(64 * AT_WAVES, sizeof(CT) == 4 && HD == 128 ? 2 : 3) void paged_attend_kernel(AttendArgs a) {
+struct AtStep {
   using Y = AtTypes<RT, CT, HD>;
-  constexpr int VW = Y::F32 ? Y::VE : Y::VE / 2;  // 32-bit words of a value lane's key
-  __shared__ f32x4 so[AT_WAVES - 1][Y::VE][64];
-  __shared__ float sm[AT_WAVES - 1][64], sl[AT_WAVES - 1][64];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-  const int hkv = a.kv.n_kv_heads, kvh = blockIdx.x % hkv;
-  int b = blockIdx.x / hkv, slot;
+  u32x4 k[Y::H][Y::KC];
+  uint32_t v[4 * Y::H][Y::VW];  // the lane's dimensions of key 4 g + (j & 3) of tile j >> 2
 
-  // The block's keys are a run [k0, k1) of one or two page lists laid end to
-  // end: the prefix up to `pre` (rounded up to a step), then the sequence's
-  // own up to `end`.  A wave has 16 columns: row, query head, own keys seen.
-  const int *ids = nullptr;
-  int pre = 0, end = 0, k0, k1, row = -1, seen = 0, waves, col, last_seen = 0;
-  if (b < a.pre_tiles * a.pre_splits) {
-    slot = b / a.pre_tiles;
-    waves = a.pre_waves;
-    const int tile = b - slot * a.pre_tiles, rows = a.row_start ? at_row(a.row_start, a.n_seqs, a.n_rows) : a.n_rows;
-    if (tile * waves * AT_COLS >= rows * a.group) return;
-    col = (tile * waves + wave % waves) * AT_COLS + c;
-    if (col < rows * a.group) row = col / a.group;
-    pre = a.prefix_len;
-    k0 = slot * a.pre_chunk;
-    k1 = min(pre, k0 + a.pre_chunk);
-  } else {
-    b -= a.pre_tiles * a.pre_splits;
-    slot = b / a.own_slots;
-    b -= slot * a.own_slots;
-    waves = a.own_waves;
-    const int tc = waves * AT_COLS;
-    int s, tile, r0, r1;
-    if (a.row_start) {
-      s = at_search(a.n_seqs, b, [&](int i) { return at_row(a.row_start, i, a.n_rows) * a.group / tc + i; });
-      if (s < 0) return;
-      r0 = at_row(a.row_start, s, a.n_rows);
-      r1 = at_row(a.row_start, s + 1, a.n_rows);
-      tile = b - (r0 * a.group / tc + s);
-    } else {
-      const int tiles = (a.group + tc - 1) / tc;
-      s = b / tiles;
-      tile = b - s * tiles;
-      r0 = s;
-      r1 = s + 1;
+  // Of the step at x: uniform addresses of the tiles and 32-bit offsets of the
+  // lanes, so that the loads take their base from scalar registers.  The empty
+  // asm keeps an offset's widening to 64 bits next to its loads: moved out of
+  // the loop, it hides from the compiler that the high half is zero, and every
+  // load's address becomes a pair of vector registers.
+  __device__ __forceinline__ void load_k(const char *pool, const AtPages &at, int x, uint32_t lane) {
+    asm volatile("" : "+v"(lane));
+#pragma unroll
+    for (int h = 0; h < Y::H; h++) {
+      const char *p = pool + at.place(x, h);
+#pragma unroll
+      for (int j = 0; j < Y::KC; j++) k[h][j] = *(const u32x4 *)(p + lane + 64 * j);
     }
-    const int cols = (r1 - r0) * a.group;
-    if (tile * tc >= cols) return;
-    col = tile * tc + wave % waves * AT_COLS + c;
-    // the j-th of n rows sees len - (n - 1 - j) keys
-    const int len = min(max(a.lens[s], 0), a.max_len + (r1 - r0)) - (r1 - r0 - 1);
-    auto sees = [&](int x) { return max(min(len + x / a.group, a.max_len), 0); };
-    last_seen = sees(min(tile * tc + tc, cols) - 1);
-    seen = sees(min(col, cols - 1));
-    if (col < cols) row = r0 + col / a.group;
-    pre = a.fused ? a.prefix_len : 0;
-    end = last_seen;
-    const int before = (pre + AT_KEYS - 1) & -AT_KEYS;
-    k0 = slot * a.own_chunk;
-    k1 = min(before + end, k0 + a.own_chunk);
-    slot += a.pre_splits;
-    const bool direct = a.pre_splits + a.own_splits == 1;
-    if (k1 <= k0 && !direct) return;
-    ids = a.table + (int64_t)s * a.table_stride;
   }
-  const int before = (pre + AT_KEYS - 1) & -AT_KEYS;
-  const int head = kvh * a.group + (row >= 0 ? col % a.group : 0);
-
-  AtWave<RT, CT, HD> w;
-  w.init(row >= 0 ? (const RT *)a.q + row * a.q_row + head * a.q_head : nullptr, a.scale);
-
-  // what the wave's column that sees least sees: keys before it need no mask
-  int least = row >= 0 ? seen : last_seen;
-  least = min(least, __shfl_xor(least, 1, 64));
-  least = min(least, __shfl_xor(least, 2, 64));
-  least = min(least, __shfl_xor(least, 4, 64));
-  least = min(least, __shfl_xor(least, 8, 64));
-  least = __builtin_amdgcn_readfirstlane(least);
-
-  // uniform base addresses, and 32-bit offsets of a lane in a tile of 16 keys
-  const char *kb = (const char *)a.kv.k + kvh * a.kv.head_stride * (int64_t)sizeof(CT);
-  const char *vb = (const char *)a.kv.v + kvh * a.kv.head_stride * (int64_t)sizeof(CT);
-  const int ts = (int)a.kv.token_stride * (int)sizeof(CT);
-  const uint32_t k_lane = c * ts + 16 * g, v_lane = 4 * g * ts + Y::VE * c * (int)sizeof(CT);
-  const int key_waves = AT_WAVES / waves, key_wave = wave / waves;
-  const int stride = AT_KEYS * key_waves;
-
-  u32x4 k[2][Y::KC];
-  uint32_t v[8][VW];
-  for (int base = k0; base < k1; base += 1024) {
-    // lane i finds the tile of keys base + 16 i .. (bytes from the pools'
-    // starts); an absent tile reads the first page, and none of it is seen
-    const int stop = min(k1, base + 1024);
-    int page = -1, slot_in = 0;
-    {
-      const int x = base + 16 * lane;
-      if (x < before) {
-        slot_in = x;
-        if (x < pre) page = pg_page(a.prefix_pages, a.prefix_count, x, a.kv.page_shift, a.kv.n_pages);
-      } else if (x < stop) {
-        slot_in = x - before;
-        page = pg_page(ids, a.table_width, slot_in, a.kv.page_shift, a.kv.n_pages);
-      }
-    }
-    const uint64_t have = __ballot(page >= 0);
-    const int64_t my_at = page < 0 ? 0 : page * a.kv.page_stride * (int64_t)sizeof(CT) + (int64_t)(slot_in & (a.kv.page_size - 1)) * ts;
-    const int at_lo = (int)my_at, at_hi = (int)(my_at >> 32);
-    auto place = [&](int x, int h) -> int64_t {
-      const int i = ((x - base) >> 4) + h;
-      return (int64_t)__builtin_amdgcn_readlane(at_hi, i) << 32 | (uint32_t)__builtin_amdgcn_readlane(at_lo, i);
-    };
-    auto load_k = [&](int x) {
+  __device__ __forceinline__ void load_v(const char *pool, const AtPages &at, int x, uint32_t lane, int ts) {
+    asm volatile("" : "+v"(lane));
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const char *p = kb + place(x, h);
+    for (int h = 0; h < Y::H; h++) {
+      const char *p = pool + at.place(x, h);
 #pragma unroll
-        for (int j = 0; j < Y::KC; j++) k[h][j] = *(const u32x4 *)(p + k_lane + 64 * j);
-      }
-    };
-    auto load_v = [&](int x) {
+      for (int i = 0; i < 4; i++, p += ts) {
+        if constexpr (Y::VW == 2) {
+          const u32x2 y = *(const u32x2 *)(p + lane);
+          v[4 * h + i][0] = y[0];
+          v[4 * h + i][1] = y[1];
+        } else {
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const char *p = vb + place(x, h);
+          for (int z = 0; z < Y::VW; z += 4) {
+            const u32x4 y = *(const u32x4 *)(p + lane + 4 * z);
 #pragma unroll
-        for (int i = 0; i < 4; i++, p += ts) {
-          if constexpr (VW == 2) {
-            const u32x2 y = *(const u32x2 *)(p + v_lane);
-            v[4 * h + i][0] = y[0];
-            v[4 * h + i][1] = y[1];
-          } else {
-#pragma unroll
-            for (int z = 0; z < VW; z += 4) {
-              const u32x4 y = *(const u32x4 *)(p + v_lane + 4 * z);
-#pragma unroll
-              for (int u = 0; u < 4; u++) v[4 * h + i][z + u] = y[u];
-            }
+            for (int u = 0; u < 4; u++) v[4 * h + i][z + u] = y[u];
           }
         }
       }
-    };
-    int x = base + AT_KEYS * key_wave;
+    }
+  }
+  // Values that no column sees (from row `any` on, or in an absent tile) may
+  // be anything, and 0 times them not 0: they are put to zero.  What is not
+  // finite from row `all` on, which not all columns see, is too, and its rows
+  // are returned.
+  __device__ __forceinline__ uint32_t clean(uint32_t there, int all, int any) {
+    const int g = (threadIdx.x & 63) >> 4;
+    uint32_t rows = 0;
+#pragma unroll
+    for (int j = 0; j < 4 * Y::H; j++) {
+      const int row = 16 * (j >> 2) + 4 * g + (j & 3);
+      const bool none = !(there >> (j >> 2) & 1) | (row >= any);
+      bool bad = false;
+#pragma unroll
+      for (int y = 0; y < Y::VW; y++) {
+        v[j][y] = none ? 0 : v[j][y];
+        bad |= at_odd<CT>(v[j][y]);
+      }
+      bad &= row >= all;
+      const uint64_t lanes = __ballot(bad);
+      if (lanes) {
+#pragma unroll
+        for (int y = 0; y < Y::VW; y++) v[j][y] = bad ? at_finite<CT>(v[j][y]) : v[j][y];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (lanes >> (16 * i) & 0xffff) rows |= 1u << (16 * (j >> 2) + 4 * i + (j & 3));
+      }
+    }
+    return rows;
+  }
+  // 16-bit caches: the A operands of value instructions 2 w and 2 w + 1
+  __device__ __forceinline__ void turn(int w, u32x4 &a, u32x4 &b) const {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {  // key pairs: the low halves, the high halves
+      a[j] = __builtin_amdgcn_perm(v[2 * j + 1][w], v[2 * j][w], 0x05040100u);
+      b[j] = __builtin_amdgcn_perm(v[2 * j + 1][w], v[2 * j][w], 0x07060302u);
+    }
+  }
+};
+
+// hides what a column does not see: keys from row `limit` on, absent tiles
+template <int N>
+__device__ __forceinline__ void at_hide(float (&p)[N], uint32_t there, int limit) {
+  const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int j = 0; j < N; j++) {
+    const bool is = (there >> (j >> 2) & 1) & (16 * (j >> 2) + 4 * g + (j & 3) < limit);
+    p[j] = is ? p[j] : -INFINITY;
+  }
+}
+
+template <typename RT, typename CT, int HD, bool WIDE>
+struct AtLds {
+  using Y = AtTypes<RT, CT, HD>;
+  static constexpr int JOIN = (AT_WAVES - 1) * Y::VE * 64;             // states of the waves that share columns
+  static constexpr int K = WIDE ? AT_WAVES * Y::H * Y::KC * 64 : 0;    // operands of a stage's keys
+  static constexpr int V = WIDE ? AT_WAVES * Y::VE * 64 : 0;           // ... and values
+  u32x4 x[JOIN > K + V ? JOIN : K + V];
+  float m[AT_WAVES - 1][64], l[AT_WAVES - 1][64];
+  uint32_t rows[AT_WAVES];  // of each step of the stage: what clean() returned
+};
+
+// Few columns: 16 a wave; waves with the same ones split the keys
+template <typename RT, typename CT, int HD>
+__device__ __forceinline__ void at_narrow(const AttendArgs &a, const AtJob &b, int cols, int kvh, u32x4 *so,
+                                          float (*sm)[64], float (*sl)[64]) {
+  using Y = AtTypes<RT, CT, HD>;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int col_waves = cols / AT_COLS, key_waves = AT_WAVES / col_waves, key_wave = wave / col_waves;
+  const int first = b.first + wave % col_waves * AT_COLS, col = first + c;
+  const int row = col < b.cols ? b.r0 + col / b.group : -1, head = kvh * b.group + col % b.group;
+  const int seen = b.sees(col), least = b.sees(first), most = b.sees(first + AT_COLS - 1);
+  AtTile<RT, CT, HD> w;
+  w.init(row >= 0 ? (const RT *)a.q + row * a.q_row + head * a.q_head : nullptr, a.scale);
+
+  const char *kb = (const char *)a.kv.k + kvh * a.kv.head_stride * (int64_t)sizeof(CT);
+  const char *vb = (const char *)a.kv.v + kvh * a.kv.head_stride * (int64_t)sizeof(CT);
+  const int ts = (int)a.kv.token_stride * (int)sizeof(CT), stride = Y::STEP * key_waves;
+  const uint32_t k_lane = c * ts + 16 * g, v_lane = 4 * g * ts + Y::VE * c * (int)sizeof(CT);
+  AtStep<RT, CT, HD> t;
+  AtPages at;
+  for (int base = b.k0; base < b.k1; base += 1024) {
+    const int stop = min(b.k1, base + 1024);
+    at.look(b, a.kv, base, stop, ts, sizeof(CT));
+    int x = base + Y::STEP * key_wave;
     if (x >= stop) continue;
-    load_k(x);
-    load_v(x);
+    t.load_k(kb, at, x, k_lane);
+    t.load_v(vb, at, x, v_lane, ts);
     // The next step's keys are asked for when this one's scores are taken, its
     // values when this one's are summed: one of the two is always on its way.
     // The last step asks for itself again, so that the number of loads in
     // flight is the same on every path and the waits can be exact.
     for (;;) {
       const int next = x + stride < stop ? x + stride : x;
-      float p[8];
+      float p[4 * Y::H];
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const f32x4 s = w.score(k[h]);
+      for (int h = 0; h < Y::H; h++) {
+        f32x4 d{0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < 4; i++) p[4 * h + i] = s[i] * w.qs;
+        for (int j = 0; j < Y::KC; j++) d = w.score(t.k[h][j], j, d);
+#pragma unroll
+        for (int i = 0; i < 4; i++) p[4 * h + i] = d[i] * w.qs;
       }
-      load_k(next);
-      const uint32_t there = (uint32_t)(have >> ((x - base) >> 4)) & 3;
-      // keys of this list that are seen: by the column, by all, by any
-      const bool shared = x < before;
-      const int x0 = shared ? x : x - before;
-      const int lim = shared ? pre : seen, all = shared ? pre : least, any = shared ? pre : end;
-      uint32_t odd = 0;  // bit j: the lane's part of key j is not finite, and not seen by all
-      if (all < x0 + AT_KEYS || there != 3) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const int key = x0 + 16 * (j >> 2) + 4 * g + (j & 3);
-          const bool is = there >> (j >> 2) & 1;
-          p[j] = is & (key < lim) ? p[j] : -INFINITY;
-          // a value that no column sees may be anything, and 0 times it not 0
-          const bool none = !is | (key >= any);
-          bool bad = false;
-#pragma unroll
-          for (int y = 0; y < VW; y++) {
-            v[j][y] = none ? 0 : v[j][y];
-            bad |= at_odd<CT>(v[j][y]);
-          }
-          odd |= (uint32_t)(bad & (key >= all)) << j;
-        }
+      t.load_k(kb, at, next, k_lane);
+      const uint32_t there = at.there(x, Y::H);
+      const bool shared = x < b.before;
+      const int x0 = shared ? x : x - b.before;  // in its list
+      uint32_t rows = 0;
+      if ((shared ? b.pre : least) < x0 + Y::STEP || there != (1u << Y::H) - 1) {
+        at_hide(p, there, (shared ? b.pre : seen) - x0);
+        rows = t.clean(there, (shared ? b.pre : least) - x0, (shared ? b.pre : most) - x0);
       }
       w.softmax(p);
-      if (__any(odd)) {
-        // such elements are taken out of the common product and added to the
-        // columns that see them one by one, each lane to its own dimensions
-        for (int j = 0; j < 8; j++) {
-          const uint64_t lanes = __ballot(odd >> j & 1);
+      if (rows) w.add_odd(rows, p, (shared ? b.pre : seen) - x0, ts, [&](int h) { return vb + at.place(x, h); });
+      if constexpr (Y::F32) {
 #pragma unroll
-          for (int jj = 0; jj < 8; jj++)
+        for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int y = 0; y < VW; y++) v[jj][y] = jj == j && (odd >> j & 1) ? at_finite<CT>(v[jj][y]) : v[jj][y];
-          float pj = p[0];
+          for (int e = 0; e < Y::VE; e++)
+            w.o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, t.v[j][e]), p[j], w.o[e], 0, 0, 0);
+      } else {
+        typename At8<CT>::T pb[Y::SPLIT ? 2 : 1];
+        w.weights(p, pb);
 #pragma unroll
-          for (int jj = 1; jj < 8; jj++) pj = jj == j ? p[jj] : pj;
-          for (int gg = 0; gg < 4; gg++) {
-            if (!(lanes >> (16 * gg) & 0xffff)) continue;
-            const int in = 4 * gg + (j & 3);
-            const float weight = __shfl(pj, 16 * gg + c, 64);
-            const CT *row = (const CT *)(vb + place(x, j >> 2) + (int64_t)in * ts) + 4 * Y::VE * g;
-            if (x0 + 16 * (j >> 2) + in < lim) {
-#pragma unroll
-              for (int i = 0; i < 4; i++) {
-                float y[Y::VE];
-                pg_load(row + Y::VE * i, y);
-#pragma unroll
-                for (int e = 0; e < Y::VE; e++)
-                  if (!(fabsf(y[e]) < INFINITY)) w.o[e][i] = fmaf(weight, y[e], w.o[e][i]);
-              }
-            }
-          }
+        for (int i = 0; i < Y::VE / 2; i++) {
+          u32x4 u, v;
+          t.turn(i, u, v);
+          w.value(2 * i, u, pb);
+          w.value(2 * i + 1, v, pb);
         }
       }
-      w.values(p, v);
-      load_v(next);
+      t.load_v(vb, at, next, v_lane, ts);
       if (next == x) break;
       x = next;
     }
   }
 
   // the waves with the same columns join their states in the first one's
-  w.l = at_sum4(w.l);
   if (key_waves > 1) {
     if (key_wave > 0) {
-      const int at = wave - waves;
+      const int i = wave - col_waves;
 #pragma unroll
-      for (int e = 0; e < Y::VE; e++) so[at][e][lane] = w.o[e];
-      sm[at][lane] = w.m;
-      sl[at][lane] = w.l;
+      for (int e = 0; e < Y::VE; e++) so[(i * Y::VE + e) * 64 + lane] = __builtin_bit_cast(u32x4, w.o[e]);
+      sm[i][lane] = w.m;
+      sl[i][lane] = w.l;
     }
     __syncthreads();
     if (key_wave > 0) return;
-    for (int i = 1; i < key_waves; i++) {
-      const int at = wave + (i - 1) * waves;
-      const float m1 = sm[at][lane], m = fmaxf(w.m, m1);
+    for (int k = 1; k < key_waves; k++) {
+      const int i = wave + (k - 1) * col_waves;
+      const float m1 = sm[i][lane], m = fmaxf(w.m, m1);
       // (a state without a maximum holds zeros, or NaN, which must not get lost)
       const float f0 = w.m == -INFINITY ? 1.0f : at_exp2(w.m - m), f1 = m1 == -INFINITY ? 1.0f : at_exp2(m1 - m);
       w.m = m;
-      w.l = w.l * f0 + sl[at][lane] * f1;
+      w.l = w.l * f0 + sl[i][lane] * f1;
 #pragma unroll
-      for (int e = 0; e < Y::VE; e++) w.o[e] = w.o[e] * f0 + so[at][e][lane] * f1;
+      for (int e = 0; e < Y::VE; e++) w.o[e] = w.o[e] * f0 + __builtin_bit_cast(f32x4, so[(i * Y::VE + e) * 64 + lane]) * f1;
     }
   }
-  if (row < 0) return;
-  // the lane's dimensions: 4 VE from 4 VE g on
-  if (a.pre_splits + a.own_splits == 1) {
-    const float r = w.l == 0 ? 0.0f : 1.0f / w.l;
-    RT *out = (RT *)a.out + row * a.o_row + head * a.o_head + 4 * Y::VE * g;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      float y[Y::VE];
-#pragma unroll
-      for (int e = 0; e < Y::VE; e++) y[e] = w.o[e][i] * r;
-      pg_store(out + Y::VE * i, y);
-    }
-    if (a.lse && g == 0) a.lse[(int64_t)row * a.n_heads + head] = at_lse(w.m, w.l);
-    return;
-  }
-  const int64_t item = ((int64_t)slot * a.n_rows + row) * a.n_heads + head;
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    float y[Y::VE];
-#pragma unroll
-    for (int e = 0; e < Y::VE; e++) y[e] = w.o[e][i];
-    pg_store(a.part_o + item * HD + 4 * Y::VE * g + Y::VE * i, y);
-  }
-  if (g == 0) a.part_ml[item] = make_float2(w.m, w.l);
+  w.store(a, b.slot, row, head);
 }
 
-// Joins a row and head's partials, a wave each: lane l takes dimensions
-// HD / 64 l ..
+// Many columns: a stage is 128 keys, 32 brought by each wave, and every wave
+// takes them all through its own columns
+template <typename RT, typename CT, int HD>
+__device__ __forceinline__ void at_wide(const AttendArgs &a, const AtJob &b, int kvh, AtLds<RT, CT, HD, true> &s) {
+  using Y = AtTypes<RT, CT, HD>;
+  constexpr int N = Y::WIDE;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int first = b.first + wave * N * AT_COLS;
+  AtTile<RT, CT, HD> w[N];
+  int row[N], head[N], seen[N];
+#pragma unroll
+  for (int n = 0; n < N; n++) {
+    const int col = first + n * AT_COLS + c;
+    row[n] = col < b.cols ? b.r0 + col / b.group : -1;
+    head[n] = kvh * b.group + col % b.group;
+    seen[n] = b.sees(col);
+    w[n].init(row[n] >= 0 ? (const RT *)a.q + row[n] * a.q_row + head[n] * a.q_head : nullptr, a.scale);
+  }
+  const int least = b.sees(first), most = b.sees(first + N * AT_COLS - 1);          // of the wave's columns
+  const int block_least = b.sees(b.first), block_most = b.sees(b.first + AT_WAVES * N * AT_COLS - 1);
+  const bool idle = first >= b.cols;
+
+  const char *kb = (const char *)a.kv.k + kvh * a.kv.head_stride * (int64_t)sizeof(CT);
+  const char *vb = (const char *)a.kv.v + kvh * a.kv.head_stride * (int64_t)sizeof(CT);
+  const int ts = (int)a.kv.token_stride * (int)sizeof(CT);
+  const uint32_t k_lane = c * ts + 16 * g, v_lane = 4 * g * ts + Y::VE * c * (int)sizeof(CT);
+  u32x4 *const sk = s.x, *const sv = s.x + AtLds<RT, CT, HD, true>::K;
+  AtStep<RT, CT, HD> t;
+  AtPages at;
+  for (int base = b.k0; base < b.k1; base += 1024) {
+    const int stop = min(b.k1, base + 1024), end = base + ((stop - 1 - base) & -AT_KEYS);  // the last step's start
+    at.look(b, a.kv, base, stop, ts, sizeof(CT));
+    auto load = [&](int from) {
+      const int x = min(from + AT_KEYS * wave, end);
+      t.load_k(kb, at, x, k_lane);
+      t.load_v(vb, at, x, v_lane, ts);
+    };
+    load(base);
+    for (int from = base; from < stop; from += AT_STAGE) {
+      {
+        const int x = min(from + AT_KEYS * wave, end);
+        const bool shared = x < b.before;
+        const int x0 = shared ? x : x - b.before;
+        const uint32_t there = at.there(x, Y::H);
+        uint32_t rows = 0;
+        if ((shared ? b.pre : block_least) < x0 + AT_KEYS || there != 3)
+          rows = t.clean(there, (shared ? b.pre : block_least) - x0, (shared ? b.pre : block_most) - x0);
+        if (lane == 0) s.rows[wave] = rows;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int j = 0; j < Y::KC; j++) sk[((wave * 2 + h) * Y::KC + j) * 64 + lane] = t.k[h][j];
+#pragma unroll
+        for (int i = 0; i < Y::VE / 2; i++) {
+          u32x4 u, v;
+          t.turn(i, u, v);
+          sv[(wave * Y::VE + 2 * i) * 64 + lane] = u;
+          sv[(wave * Y::VE + 2 * i + 1) * 64 + lane] = v;
+        }
+      }
+      __syncthreads();
+      if (from + AT_STAGE < stop) load(from + AT_STAGE);
+      for (int i = 0; i < AT_WAVES; i++) {
+        const int x = from + AT_KEYS * i;
+        const bool shared = x < b.before;
+        const int x0 = shared ? x : x - b.before;
+        if (x >= stop || idle || (!shared && x0 >= most)) break;
+        const uint32_t there = at.there(x, Y::H);
+        float p[N][8];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          f32x4 d[N];
+#pragma unroll
+          for (int n = 0; n < N; n++) d[n] = f32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < Y::KC; j++) {
+            const u32x4 k = sk[((i * 2 + h) * Y::KC + j) * 64 + lane];
+#pragma unroll
+            for (int n = 0; n < N; n++) d[n] = w[n].score(k, j, d[n]);
+          }
+#pragma unroll
+          for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int u = 0; u < 4; u++) p[n][4 * h + u] = d[n][u] * w[n].qs;
+        }
+        const uint32_t rows = __builtin_amdgcn_readfirstlane(s.rows[i]);
+        if ((shared ? b.pre : least) < x0 + AT_KEYS || there != 3) {
+#pragma unroll
+          for (int n = 0; n < N; n++) at_hide(p[n], there, (shared ? b.pre : seen[n]) - x0);
+        }
+        typename At8<CT>::T pb[N][Y::SPLIT ? 2 : 1];
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+          w[n].softmax(p[n]);
+          w[n].weights(p[n], pb[n]);
+        }
+        if (rows) {
+#pragma unroll
+          for (int n = 0; n < N; n++)
+            w[n].add_odd(rows, p[n], (shared ? b.pre : seen[n]) - x0, ts, [&](int h) { return vb + at.place(x, h); });
+        }
+#pragma unroll
+        for (int e = 0; e < Y::VE; e++) {
+          const u32x4 v = sv[(i * Y::VE + e) * 64 + lane];
+#pragma unroll
+          for (int n = 0; n < N; n++) w[n].value(e, v, pb[n]);
+        }
+      }
+      __syncthreads();
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < N; n++) w[n].store(a, b.slot, row[n], head[n]);
+}
+
+// WIDE: some of the blocks are wide; their registers and 64 KB of LDS allow 2
+// waves on a SIMD, narrow blocks alone 3 (16 KB in flight a wave).
+template <typename RT, typename CT, int HD, bool WIDE>
+__global__ __launch_bounds__(64 * AT_WAVES, 2) void paged_attend_kernel(AttendArgs a) {
+  __shared__ AtLds<RT, CT, HD, WIDE> lds;
+  const int hkv = a.kv.n_kv_heads, kvh = blockIdx.x % hkv;
+  int i = blockIdx.x / hkv;
+  AtJob b{};
+  b.prefix_ids = a.prefix_pages;
+  b.n_prefix_ids = a.prefix_count;
+  b.group = a.group;
+  b.max_len = a.max_len;
+  bool wide;
+  int cols;  // of the block
+  if (i < a.pre_tiles * a.pre_splits) {
+    wide = a.pre_wide;
+    cols = a.pre_cols;
+    b.slot = i / a.pre_tiles;
+    b.first = (i - b.slot * a.pre_tiles) * cols;
+    b.cols = (a.row_start ? at_row(a.row_start, a.n_seqs, a.n_rows) : a.n_rows) * a.group;
+    if (b.first >= b.cols) return;
+    b.pre = a.prefix_len;
+    b.before = (b.pre + AT_KEYS - 1) & -AT_KEYS;
+    b.k0 = b.slot * a.pre_chunk;
+    b.k1 = min(b.pre, b.k0 + a.pre_chunk);
+  } else {
+    wide = a.own_wide;
+    cols = a.own_cols;
+    i -= a.pre_tiles * a.pre_splits;
+    const int split = i / a.own_slots;
+    i -= split * a.own_slots;
+    int s, tile, rows = 1;
+    if (a.row_start) {
+      s = at_search(a.n_seqs, i, [&](int x) { return at_row(a.row_start, x, a.n_rows) * a.group / cols + x; });
+      if (s < 0) return;
+      b.r0 = at_row(a.row_start, s, a.n_rows);
+      rows = at_row(a.row_start, s + 1, a.n_rows) - b.r0;
+      tile = i - (b.r0 * a.group / cols + s);
+    } else {
+      const int tiles = (a.group + cols - 1) / cols;
+      b.r0 = s = i / tiles;
+      tile = i - s * tiles;
+    }
+    b.slot = a.pre_splits + split;
+    b.first = tile * cols;
+    b.cols = rows * a.group;
+    if (b.first >= b.cols) return;
+    // the j-th of n rows sees lens - (n - 1 - j) keys
+    b.len = min(max(a.lens[s], 0), a.max_len + rows) - (rows - 1);
+    b.pre = a.fused ? a.prefix_len : 0;
+    b.before = (b.pre + AT_KEYS - 1) & -AT_KEYS;
+    b.ids = a.table + (int64_t)s * a.table_stride;
+    b.n_ids = a.table_width;
+    b.k0 = split * a.own_chunk;
+    const int end = b.sees(b.first + cols - 1);
+    b.k1 = min(end ? b.before + end : b.pre, b.k0 + a.own_chunk);
+    // an empty split is not read by the join; alone, it writes zeros
+    if (b.k1 <= b.k0 && a.pre_splits + a.own_splits > 1) return;
+  }
+  if constexpr (WIDE) {
+    if (wide) {
+      at_wide<RT, CT, HD>(a, b, kvh, lds);
+      return;
+    }
+  }
+  at_narrow<RT, CT, HD>(a, b, cols, kvh, lds.x, lds.m, lds.l);
+}
+
+// Joins a row and head's partials: a wave each, or the four waves of a block
+// where there are many.  Lane l takes dimensions HD / 64 l ..
 template <typename RT, int HD>
-__global__ __launch_bounds__(256) void paged_attend_join_kernel(AttendArgs a) {
-  constexpr int N = HD / 64;
-  const int lane = threadIdx.x & 63;
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), items = (int64_t)a.n_rows * a.n_heads;
+__global__ __launch_bounds__(64 * AT_WAVES) void paged_attend_join_kernel(AttendArgs a) {
+  constexpr int N = HD / 64, VE = HD / 16;
+  __shared__ float sy[AT_WAVES][HD], sl[AT_WAVES];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t items = (int64_t)a.n_rows * a.n_heads;
+  const int64_t item = a.team > 1 ? blockIdx.x : (int64_t)blockIdx.x * AT_WAVES + wave;
   if (item >= items) return;
   const int row = (int)(item / a.n_heads), head = (int)(item - (int64_t)row * a.n_heads);
   int s = row, back = 0;  // back: rows of the sequence behind this one
@@ -774,22 +979,40 @@ __global__ __launch_bounds__(256) void paged_attend_join_kernel(AttendArgs a) {
     back = end - 1 - row;
   }
   const int seen = min(min(max(a.lens[s], 0), a.max_len + back + 1) - back, a.max_len);
-  const int own = seen > 0 ? (seen + a.own_chunk - 1) / a.own_chunk : 0;
-  const int parts = a.pre_splits + own;
+  const int pre = a.fused ? a.prefix_len : 0, before = (pre + AT_KEYS - 1) & -AT_KEYS;
+  const int keys = seen > 0 ? before + seen : pre;
+  const int parts = a.pre_splits + (keys > 0 ? (keys + a.own_chunk - 1) / a.own_chunk : 0);
   float m = -INFINITY;
   for (int i = lane; i < parts; i += 64) m = fmaxf(m, a.part_ml[i * items + item].x);
   m = wave_max(m);
+  // the lane's dimensions N l + j lie at 16 e + r, VE r + e = N l + j
+  const int at = N * lane % VE * 16 + N * lane / VE;
   float l = 0, y[N];
 #pragma unroll
   for (int j = 0; j < N; j++) y[j] = 0;
-  for (int i = 0; i < parts; i++) {
+  const int first = a.team > 1 ? wave : 0;
+#pragma unroll 4
+  for (int i = first; i < parts; i += a.team) {
     const float2 ml = a.part_ml[i * items + item];
+    const float *o = a.part_o + (i * items + item) * HD + at;
+    // (a part without a maximum holds zeros, or NaN, which must not get lost)
     const float f = ml.x == -INFINITY ? 1.0f : at_exp2(ml.x - m);
-    float x[N];
-    pg_load(a.part_o + (i * items + item) * HD + N * lane, x);
     l = fmaf(ml.y, f, l);
 #pragma unroll
-    for (int j = 0; j < N; j++) y[j] = fmaf(x[j], f, y[j]);
+    for (int j = 0; j < N; j++) y[j] = fmaf(o[16 * j], f, y[j]);
+  }
+  if (a.team > 1) {
+#pragma unroll
+    for (int j = 0; j < N; j++) sy[wave][N * lane + j] = y[j];
+    if (lane == 0) sl[wave] = l;
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int u = 1; u < AT_WAVES; u++) {
+      l += sl[u];
+#pragma unroll
+      for (int j = 0; j < N; j++) y[j] += sy[u][N * lane + j];
+    }
   }
   const float r = l == 0 ? 0.0f : 1.0f / l;
 #pragma unroll
