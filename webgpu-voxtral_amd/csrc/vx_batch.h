@@ -120,8 +120,14 @@ inline int paged_append(const vx_append_args *p, void *stream) {
   a.pos = p->pos, a.seq = p->seq, a.table = p->table, a.table_stride = p->table_stride;
   a.table_width = p->table_width, a.base = p->base, a.n_tokens = p->n_tokens, a.n_seqs = p->n_seqs;
   a.n_heads = p->n_heads, a.head_dim = p->kv.head_dim, a.rotary_dim = p->rotary_dim, a.interleaved = p->interleaved;
+  // theta^(-2 i / rotary_dim) as a product of two of 16 powers
   const double step = p->rotary_dim ? -2.0 * std::log2(p->theta) / p->rotary_dim : 0;
-  for (int i = 0; i < 64; i++) a.turns[i] = i < p->rotary_dim / 2 ? std::exp2(i * step) * 0.15915494309189533577 : 0;
+  double low[8];
+  for (int i = 0; i < 8; i++) low[i] = std::exp2(i * step);
+  for (int i = 0; i < 64; i += 8) {
+    const double high = i < p->rotary_dim / 2 ? std::exp2(i * step) * 0.15915494309189533577 : 0;
+    for (int j = 0; j < 8; j++) a.turns[i + j] = high * low[j];
+  }
   OnDevice on(p->kv.device);
   if (on.status != hipSuccess) return batch_fail(VX_E_DEVICE, "%s: device %d: %s", what, p->kv.device, hipGetErrorString(on.status));
   return with_types(p->type, p->kv.type, [&](auto r, auto c) {

@@ -24,13 +24,17 @@ assert _KV.size == 64
 
 _torch = None
 _types = None  # dtype -> VX_TYPE_*
+_raw_stream = None
 
 
 def _load():
-    global _torch, _types
+    global _torch, _types, _raw_stream
     if _torch is None:
         import torch
         _types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+        # the number of the current stream, without an object around it (2 us less a call)
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                              lambda index: torch.cuda.current_stream(index).cuda_stream)
         _torch = torch
     return load_library()
 
@@ -41,32 +45,43 @@ def _call(fn, *args):
         raise VoxtralError(rc, load_library().vx_batch_error().decode())
 
 
-def _stream(device, stream):
-    if stream is None:
-        return _torch.cuda.current_stream(device).cuda_stream
-    return getattr(stream, "cuda_stream", stream)
+def _stream(index, stream):
+    return _raw_stream(index) if stream is None else getattr(stream, "cuda_stream", stream)
 
 
-def _tensor(name, x, dims, device):
-    """x checked: a tensor of `dims` dimensions on `device`, its last one contiguous."""
+def _refuse(name, x, dims, index):
+    """Says what is wrong with x, of which _fits() is not true."""
     if not isinstance(x, _torch.Tensor):
         raise TypeError(f"{name}: a torch tensor is needed, not {type(x).__name__}")
-    if x.device != device or device.type != "cuda":
-        raise ValueError(f"{name} is on {x.device}, not on the GPU {device}")
+    if x.get_device() != index or index < 0:
+        raise ValueError(f"{name} is on {x.device}, not on GPU {index}")
     if x.dim() != dims:
         raise ValueError(f"{name} has {x.dim()} dimensions, not {dims}")
-    if x.shape[-1] > 1 and x.stride(-1) != 1:
-        raise ValueError(f"{name}: the last dimension is not contiguous")
-    if x.requires_grad and _torch.is_grad_enabled():
+    if x.requires_grad:
         raise ValueError(f"{name} requires a gradient: this operator has no backward pass")
+    raise ValueError(f"{name}: the last dimension is not contiguous")
+
+
+def _fits(x, dims, index):
+    """Whether x is a tensor of `dims` dimensions on GPU `index`, its last one contiguous."""
+    if not isinstance(x, _torch.Tensor) or x.get_device() != index or index < 0:
+        return False
+    st = x.stride()
+    return len(st) == dims and (st[-1] == 1 or x.shape[-1] <= 1) and not (x.requires_grad and _torch.is_grad_enabled())
+
+
+def _tensor(name, x, dims, index):
+    if not _fits(x, dims, index):
+        _refuse(name, x, dims, index)
     return x
 
 
-def _ints(name, x, n, device):
-    """The address of a contiguous int32 vector of n elements."""
-    _tensor(name, x, 1, device)
-    if x.dtype != _torch.int32:
-        raise TypeError(f"{name}: int32 is needed, not {x.dtype}")
+def _vector(name, x, dtype, n, index):
+    """The address of a contiguous vector of n elements (None: any number)."""
+    if not _fits(x, 1, index):
+        _refuse(name, x, 1, index)
+    if x.dtype != dtype:
+        raise TypeError(f"{name}: {dtype} is needed, not {x.dtype}")
     if n is not None and x.shape[0] != n:
         raise ValueError(f"{name} has {x.shape[0]} elements, not {n}")
     return x.data_ptr()
@@ -81,31 +96,37 @@ class PagedKV:
 
     def __init__(self, k_pages, v_pages):
         self._lib = _load()
-        self.device = getattr(k_pages, "device", None)
-        _tensor("k_pages", k_pages, 4, self.device)
-        _tensor("v_pages", v_pages, 4, self.device)
+        self.index = k_pages.get_device() if isinstance(k_pages, _torch.Tensor) else -1
+        _tensor("k_pages", k_pages, 4, self.index)
+        _tensor("v_pages", v_pages, 4, self.index)
         if v_pages.shape != k_pages.shape or v_pages.stride() != k_pages.stride() or v_pages.dtype != k_pages.dtype:
             raise ValueError("k_pages and v_pages differ in shape, strides or type")
         if k_pages.dtype not in _types:
             raise TypeError(f"k_pages: float32, float16 or bfloat16 is needed, not {k_pages.dtype}")
         self.k_pages, self.v_pages = k_pages, v_pages
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k_pages.shape
+        self._int32 = _torch.int32
         self._head = _KV.pack(k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], self.n_pages, self.page_size,
-                              self.n_kv_heads, self.head_dim, _types[k_pages.dtype], self.device.index or 0)
+                              self.n_kv_heads, self.head_dim, _types[k_pages.dtype], self.index)
 
     def _rows(self, name, x, tokens, heads):
-        _tensor(name, x, 3, self.device)
+        """The address and the strides of rows [tokens][heads][head_dim] (None: any number)."""
+        if not _fits(x, 3, self.index):
+            _refuse(name, x, 3, self.index)
         if x.dtype not in _types:
             raise TypeError(f"{name}: float32, float16 or bfloat16 is needed, not {x.dtype}")
-        if x.shape[2] != self.head_dim or (tokens is not None and x.shape[0] != tokens) or (heads is not None and x.shape[1] != heads):
+        t, h, d = x.shape
+        if d != self.head_dim or (tokens is not None and t != tokens) or (heads is not None and h != heads):
             raise ValueError(f"{name} has shape {tuple(x.shape)}, not ({tokens}, {heads}, {self.head_dim})")
-        return x
+        row, head, _ = x.stride()
+        return x.data_ptr(), row, head
 
     def _table(self, table):
-        _tensor("table", table, 2, self.device)
-        if table.dtype != _torch.int32:
+        if not _fits(table, 2, self.index):
+            _refuse("table", table, 2, self.index)
+        if table.dtype != self._int32:
             raise TypeError(f"table: int32 is needed, not {table.dtype}")
-        return table
+        return table.data_ptr(), table.stride(0)
 
     def append(self, k, v, pos, table, seq=None, base=0, q=None, q_out=None, theta=1e6, rotary_dim=None, interleaved=True,
                stream=None):
@@ -116,28 +137,29 @@ class PagedKV:
         with a negative pos, a seq outside the table or a slot without a page
         are skipped.  Returns q_out (None without q; made, with zeros for
         skipped tokens, if not given)."""
-        k = self._rows("k", k, None, self.n_kv_heads)
+        k_at, k_row, k_head = self._rows("k", k, None, self.n_kv_heads)
         n = k.shape[0]
-        v = self._rows("v", v, n, self.n_kv_heads)
-        table = self._table(table)
-        if v.dtype != k.dtype:
-            raise TypeError(f"v is {v.dtype}, k is {k.dtype}")
-        heads, qs = 0, (0, 0, 0, 0, 0, 0)
+        v_at, v_row, v_head = self._rows("v", v, n, self.n_kv_heads)
+        table_at, table_row = self._table(table)
+        seqs, width = table.shape
+        dtype = k.dtype
+        if v.dtype != dtype:
+            raise TypeError(f"v is {v.dtype}, k is {dtype}")
+        heads = q_at = q_row = q_head = o_at = o_row = o_head = 0
         if q is not None:
-            q = self._rows("q", q, n, None)
+            q_at, q_row, q_head = self._rows("q", q, n, None)
             heads = q.shape[1]
             if q_out is None:
                 q_out = q.new_zeros(q.shape)
-            else:
-                self._rows("q_out", q_out, n, heads)
-            if q.dtype != k.dtype or q_out.dtype != k.dtype:
-                raise TypeError(f"q is {q.dtype}, q_out is {q_out.dtype}, k is {k.dtype}")
-            qs = (q.data_ptr(), q_out.data_ptr(), q.stride(0), q.stride(1), q_out.stride(0), q_out.stride(1))
-        args = _APPEND.pack(self._head, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), *qs,
-                            _ints("pos", pos, n, self.device), 0 if seq is None else _ints("seq", seq, n, self.device),
-                            table.data_ptr(), table.stride(0), table.shape[1], base, n, table.shape[0], heads, _types[k.dtype],
-                            theta, self.head_dim if rotary_dim is None else rotary_dim, bool(interleaved))
-        _call(self._lib.vx_paged_append, args, _stream(self.device, stream))
+            o_at, o_row, o_head = self._rows("q_out", q_out, n, heads)
+            if q.dtype != dtype or q_out.dtype != dtype:
+                raise TypeError(f"q is {q.dtype}, q_out is {q_out.dtype}, k is {dtype}")
+        i32 = self._int32
+        _call(self._lib.vx_paged_append,
+              _APPEND.pack(self._head, k_at, v_at, k_row, k_head, v_row, v_head, q_at, o_at, q_row, q_head, o_row, o_head,
+                           _vector("pos", pos, i32, n, self.index), 0 if seq is None else _vector("seq", seq, i32, n, self.index),
+                           table_at, table_row, width, base, n, seqs, heads, _types[dtype], theta,
+                           self.head_dim if rotary_dim is None else rotary_dim, bool(interleaved)), _stream(self.index, stream))
         return q_out if q is not None else None
 
     def attend(self, q, lens, table, row_start=None, prefix_pages=None, prefix_len=0, max_len=None, scale=None, out=None,
@@ -153,51 +175,50 @@ class PagedKV:
         (made if not given, with zeros in rows behind the last sequence).
         workspace: a uint8 tensor of attend_workspace() bytes for this call
         alone (None: made by this call)."""
-        q = self._rows("q", q, None, None)
-        n, heads = q.shape[0], q.shape[1]
-        table = self._table(table)
+        q_at, q_row, q_head = self._rows("q", q, None, None)
+        n, heads, _ = q.shape
+        table_at, table_row = self._table(table)
         seqs, width = table.shape
-        lens_at = _ints("lens", lens, seqs, self.device)
-        start = 0 if row_start is None else _ints("row_start", row_start, seqs + 1, self.device)
+        i32, index = self._int32, self.index
+        lens_at = _vector("lens", lens, i32, seqs, index)
+        start = 0 if row_start is None else _vector("row_start", row_start, i32, seqs + 1, index)
         pages, count = 0, 0
         if prefix_pages is not None:
-            pages = _ints("prefix_pages", prefix_pages, None, self.device)
+            pages = _vector("prefix_pages", prefix_pages, i32, None, index)
             count = prefix_pages.shape[0]
         if max_len is None:
             max_len = width * self.page_size
         if out is None:
             out = q.new_empty(q.shape) if row_start is None else q.new_zeros(q.shape)
-        else:
-            self._rows("out", out, n, heads)
-            if out.dtype != q.dtype:
-                raise TypeError(f"out is {out.dtype}, q is {q.dtype}")
+        o_at, o_row, o_head = self._rows("out", out, n, heads)
+        if out.dtype != q.dtype:
+            raise TypeError(f"out is {out.dtype}, q is {q.dtype}")
+        lse_at = 0
         if lse is not None:
-            _tensor("lse", lse, 2, self.device)
+            _tensor("lse", lse, 2, index)
             if lse.dtype != _torch.float32 or lse.shape != (n, heads) or not lse.is_contiguous():
                 raise ValueError(f"lse: a contiguous float32 tensor of shape ({n}, {heads}) is needed")
+            lse_at = lse.data_ptr()
         if scale is None:
             scale = 0.0
         elif scale == 0:
             raise ValueError("scale is 0")
-
-        def pack(at, size):
-            return _ATTEND.pack(self._head, q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), q.stride(0),
-                                q.stride(1), out.stride(0), out.stride(1), start, lens_at, table.data_ptr(), pages,
-                                table.stride(0), width, count, prefix_len, max_len, n, seqs, heads, _types[q.dtype], scale, at,
-                                size)
-
+        args = [self._head, q_at, o_at, lse_at, q_row, q_head, o_row, o_head, start, lens_at, table_at, pages, table_row, width, count,
+                prefix_len, max_len, n, seqs, heads, _types[q.dtype], scale, 0, 0]
         if workspace is None:
             need = ctypes.c_size_t()
-            _call(self._lib.vx_paged_attend_workspace, pack(0, 0), ctypes.byref(need))
-            # on the stream's own terms: torch's allocator orders its reuse by the current stream
-            workspace = table.new_empty((need.value + 3) // 4)
-            if stream is not None and need.value:
-                workspace.record_stream(stream if isinstance(stream, _torch.cuda.Stream)
-                                        else _torch.cuda.ExternalStream(_stream(self.device, stream), self.device))
+            _call(self._lib.vx_paged_attend_workspace, _ATTEND.pack(*args), ctypes.byref(need))
+            if need.value:
+                # torch's allocator orders its reuse by the current stream
+                workspace = table.new_empty((need.value + 3) // 4)
+                if stream is not None:
+                    workspace.record_stream(stream if isinstance(stream, _torch.cuda.Stream)
+                                            else _torch.cuda.ExternalStream(_stream(index, stream), index))
         else:
-            _tensor("workspace", workspace, 1, self.device)
-        _call(self._lib.vx_paged_attend, pack(workspace.data_ptr(), workspace.numel() * workspace.element_size()),
-              _stream(self.device, stream))
+            _tensor("workspace", workspace, 1, index)
+        if workspace is not None:
+            args[-2], args[-1] = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        _call(self._lib.vx_paged_attend, _ATTEND.pack(*args), _stream(index, stream))
         return out
 
     def attend_workspace(self, rows, heads, seqs, width, ragged=False, prefix_len=0, max_len=None, dtype=None):
@@ -225,33 +246,31 @@ def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=N
     probability among them; a row with nothing but NaN and -inf gives (-1, 0,
     0).  out: these three tensors, to write to."""
     lib = _load()
-    device = getattr(logits, "device", None)
-    _tensor("logits", logits, 2, device)
+    index = logits.get_device() if isinstance(logits, _torch.Tensor) else -1
+    _tensor("logits", logits, 2, index)
     if logits.dtype not in _types:
         raise TypeError(f"logits: float32, float16 or bfloat16 is needed, not {logits.dtype}")
     rows, n = logits.shape
-
-    def vector(name, x, dtype):
-        _tensor(name, x, 1, device)
-        if x.dtype != dtype:
-            raise TypeError(f"{name}: {dtype} is needed, not {x.dtype}")
-        if x.shape[0] != rows:
-            raise ValueError(f"{name} has {x.shape[0]} elements, not {rows}")
-        return x.data_ptr()
-
-    def setting(name, x, dtype):
-        return (vector(name, x, dtype), 0) if isinstance(x, _torch.Tensor) else (0, x)
-
-    f32, i32 = _torch.float32, _torch.int32
-    temperature, t0 = setting("temperature", temperature, f32)
-    top_k, k0 = setting("top_k", top_k, i32)
-    top_p, p0 = setting("top_p", top_p, f32)
-    min_p, m0 = setting("min_p", min_p, f32)
+    f32, i32, tensor = _torch.float32, _torch.int32, _torch.Tensor
+    t_at = k_at = p_at = m_at = 0
+    if isinstance(temperature, tensor):
+        t_at, temperature = _vector("temperature", temperature, f32, rows, index), 0
+    if isinstance(top_k, tensor):
+        k_at, top_k = _vector("top_k", top_k, i32, rows, index), 0
+    if isinstance(top_p, tensor):
+        p_at, top_p = _vector("top_p", top_p, f32, rows, index), 0
+    if isinstance(min_p, tensor):
+        m_at, min_p = _vector("min_p", min_p, f32, rows, index), 0
+    u_at = _vector("u", u, _torch.float64, rows, index)
     if out is None:
-        out = logits.new_empty(rows, dtype=i32), logits.new_empty(rows, dtype=i32), logits.new_empty(rows, dtype=f32)
-    token, kept, prob = out
-    _call(lib.vx_sample_rows,
-          _SAMPLE.pack(logits.data_ptr(), logits.stride(0), temperature, top_p, min_p, top_k, vector("u", u, _torch.float64),
-                       vector("token", token, i32), vector("kept", kept, i32), vector("prob", prob, f32), rows, n,
-                       _types[logits.dtype], device.index or 0, t0, p0, m0, k0), _stream(device, stream))
+        token = logits.new_empty(rows, dtype=i32)
+        kept = logits.new_empty(rows, dtype=i32)
+        prob = logits.new_empty(rows, dtype=f32)
+        at = token.data_ptr(), kept.data_ptr(), prob.data_ptr()
+    else:
+        token, kept, prob = out
+        at = (_vector("token", token, i32, rows, index), _vector("kept", kept, i32, rows, index),
+              _vector("prob", prob, f32, rows, index))
+    _call(lib.vx_sample_rows, _SAMPLE.pack(logits.data_ptr(), logits.stride(0), t_at, p_at, m_at, k_at, u_at, *at, rows, n,
+                                           _types[logits.dtype], index, temperature, top_p, min_p, top_k), _stream(index, stream))
     return token, kept, prob
