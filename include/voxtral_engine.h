@@ -467,8 +467,13 @@ typedef struct vx_sample_args {
   int32_t rows, n, type, device;
   float temperature0, top_p0, min_p0;
   int32_t top_k0;
+  void *workspace;                         /* aligned to 16 bytes; NULL if 0 are needed */
+  size_t workspace_bytes;
 } vx_sample_args;
 int vx_sample_rows(const vx_sample_args *a, void *stream);
+/* The bytes of workspace that a call with this type, rows and n needs (0
+ * unless a few long rows are dealt to several blocks each). */
+int vx_sample_rows_workspace(const vx_sample_args *a, size_t *bytes);
 
 /* ------------------------------------------------------ measurement */
 /* No reference counterparts (the reference times on the CPU,

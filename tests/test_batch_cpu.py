@@ -43,7 +43,7 @@ def attend(cache=None, f="vx_paged_attend", **kw):
 
 def sample(**kw):
     a = dict(logits=P, row_stride=100, temperature=0, top_p=0, min_p=0, top_k=0, u=P, token=P, kept=0, prob=0, rows=2, n=100, type=0,
-             device=0, temperature0=1.0, top_p0=1.0, min_p0=0.0, top_k0=0)
+             device=0, temperature0=1.0, top_p0=1.0, min_p0=0.0, top_k0=0, workspace=0, workspace_bytes=0)
     assert set(kw) <= set(a)
     a.update(kw)
     return V.load_library().vx_sample_rows(B._SAMPLE.pack(*a.values()), None)
@@ -97,6 +97,8 @@ def error():
     (lambda: sample(top_k0=-1), "top_k -1"),
     (lambda: sample(u=0), "NULL argument"),
     (lambda: sample(logits=P + 2), "aligned to their type"),
+    (lambda: sample(n=131072), "workspace of 0 bytes"),
+    (lambda: sample(n=131072, workspace=P + 4, workspace_bytes=1 << 30), "aligned to 16"),
 ])
 def test_refusals(call, text):
     assert call() in (V.VX_E_INVALID, V.VX_E_RANGE)
@@ -134,6 +136,13 @@ def test_workspace_covers_every_partial():
     assert rc == V.VX_OK and n >= 2 * 3 * 32 * (128 + 2) * 4
     assert attend(f="vx_paged_attend_workspace") == (V.VX_OK, 0)  # one split in all: no partials
     assert attend(f="vx_paged_attend_workspace", prefix_len=0, max_len=0) == (V.VX_OK, 0)
+
+
+def test_sample_workspace_by_sizes():
+    L = V.load_library()
+    assert L.vx_sample_rows_workspace(None, None) == V.VX_E_INVALID
+    sizes = [B._sample_space(L, rows, n, kind, 0) for rows, n, kind in ((1, 8320, 0), (500, 131072, 2), (8, 131072, 0), (1, 1 << 20, 1))]
+    assert sizes[:2] == [0, 0] and sizes[2] == 8 * sizes[3] > 0
 
 
 PROGRAM = r"""

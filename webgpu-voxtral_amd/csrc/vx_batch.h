@@ -217,12 +217,33 @@ inline int paged_attend(const vx_attend_args *p, void *stream) {
   });
 }
 
-inline int sample_rows(const vx_sample_args *p, void *stream) {
-  const char *what = "vx_sample_rows";
+inline int check_sample(const char *what, const vx_sample_args *p, SamplePlan *plan) {
   if (!p) return batch_fail(VX_E_INVALID, "%s: NULL arguments", what);
   if (!type_ok(p->type)) return batch_fail(VX_E_INVALID, "%s: logits of type %d", what, p->type);
   if (p->rows < 0 || p->n < 1) return batch_fail(VX_E_INVALID, "%s: %d rows of %d logits", what, p->rows, p->n);
   if (p->n > SR_MAXN) return batch_fail(VX_E_RANGE, "%s: %d logits a row, more than %d", what, p->n, SR_MAXN);
+  const int cus = device_cus(p->device);
+  *plan = type_size(p->type) == 4 ? sample_plan<float>(p->rows, p->n, cus) : sample_plan<_Float16>(p->rows, p->n, cus);
+  return VX_OK;
+}
+
+template <typename T>
+inline int sample_launch(const char *what, const SamplePlan &plan, const SampleArgs &a, void *stream) {
+  using H = SrHold<T>;
+  if (!plan.chunks)
+    return batch_launch(what, plan.held ? sample_held_kernel<T, H::U> : sample_rows_kernel<T>, a.rows, SR_NT, 0, a, stream);
+  const int64_t blocks = (int64_t)a.rows * plan.chunks;
+  int rc = batch_launch(what, sample_range_kernel<T, H::SPLIT_U>, blocks, SR_NT, 0, a, stream);
+  if (!rc) rc = batch_launch(what, sample_bins_kernel<T, H::SPLIT_U>, blocks, SR_NT, 0, a, stream);
+  if (!rc) rc = batch_launch(what, sample_gather_kernel<T, H::SPLIT_U>, blocks, SR_NT, 0, a, stream);
+  if (!rc) rc = batch_launch(what, sample_finish_kernel<T>, a.rows, SR_NT, 0, a, stream);
+  return rc;
+}
+
+inline int sample_rows(const vx_sample_args *p, void *stream) {
+  const char *what = "vx_sample_rows";
+  SamplePlan plan;
+  if (int rc = check_sample(what, p, &plan)) return rc;
   if (!p->temperature && !(std::isfinite(p->temperature0) && p->temperature0 >= 0))
     return batch_fail(VX_E_INVALID, "%s: temperature %g", what, p->temperature0);
   if (!p->top_p && !(p->top_p0 > 0 && p->top_p0 <= 1)) return batch_fail(VX_E_INVALID, "%s: top_p %g", what, p->top_p0);
@@ -231,18 +252,16 @@ inline int sample_rows(const vx_sample_args *p, void *stream) {
   if (p->rows == 0) return VX_OK;
   if (!p->logits || !p->u || !p->token) return batch_fail(VX_E_INVALID, "%s: NULL argument", what);
   if ((uintptr_t)p->logits % type_size(p->type)) return batch_fail(VX_E_INVALID, "%s: logits are not aligned to their type", what);
+  if (plan.bytes > p->workspace_bytes || (plan.bytes && (!p->workspace || ((uintptr_t)p->workspace & 15))))
+    return batch_fail(VX_E_INVALID, "%s: workspace of %zu bytes, %zu needed (aligned to 16)", what, p->workspace_bytes, plan.bytes);
   const SampleArgs a{p->logits, p->row_stride, p->rows, p->n, p->temperature, p->top_p, p->min_p, p->top_k, p->u,
-                     p->temperature0, p->top_p0, p->min_p0, p->top_k0, p->token, p->kept, p->prob};
+                     p->temperature0, p->top_p0, p->min_p0, p->top_k0, p->token, p->kept, p->prob,
+                     plan.chunks, plan.chunk, (char *)p->workspace};
   OnDevice on(p->device);
   if (on.status != hipSuccess) return batch_fail(VX_E_DEVICE, "%s: device %d: %s", what, p->device, hipGetErrorString(on.status));
-  auto go = [&](void (*kernel)(SampleArgs)) {
-    const hipError_t s = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, sizeof(SrShared));
-    if (s != hipSuccess) return batch_fail(VX_E_DEVICE, "%s: LDS size rejected: %s", what, hipGetErrorString(s));
-    return batch_launch(what, kernel, a.rows, SR_NT, sizeof(SrShared), a, stream);
-  };
-  return p->type == VX_TYPE_F32 ? go(sample_rows_kernel<float>)
-         : p->type == VX_TYPE_F16 ? go(sample_rows_kernel<_Float16>)
-                                  : go(sample_rows_kernel<__bf16>);
+  return p->type == VX_TYPE_F32 ? sample_launch<float>(what, plan, a, stream)
+         : p->type == VX_TYPE_F16 ? sample_launch<_Float16>(what, plan, a, stream)
+                                  : sample_launch<__bf16>(what, plan, a, stream);
 }
 
 }  // namespace vx

@@ -2520,4 +2520,12 @@ int vx_paged_attend_workspace(const vx_attend_args *a, size_t *bytes) {
 
 int vx_sample_rows(const vx_sample_args *a, void *stream) { return sample_rows(a, stream); }
 
+int vx_sample_rows_workspace(const vx_sample_args *a, size_t *bytes) {
+  if (!bytes) return batch_fail(VX_E_INVALID, "vx_sample_rows_workspace: NULL argument");
+  SamplePlan plan;
+  if (int rc = check_sample("vx_sample_rows_workspace", a, &plan)) return rc;
+  *bytes = plan.bytes;
+  return VX_OK;
+}
+
 }  // extern "C"

@@ -134,6 +134,7 @@ _SIGS = {
     "vx_paged_attend": (_I32, [ctypes.c_char_p, _VP]),
     "vx_paged_attend_workspace": (_I32, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_size_t)]),
     "vx_sample_rows": (_I32, [ctypes.c_char_p, _VP]),
+    "vx_sample_rows_workspace": (_I32, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_size_t)]),
 }
 
 _lib = None

@@ -19,7 +19,7 @@ from . import VX_OK, VoxtralError, load_library
 _KV = struct.Struct("@PPqqqiiiiii")
 _APPEND = struct.Struct("@64sPPqqqqPPqqqqPPPqiiiiiidii")
 _ATTEND = struct.Struct("@64sPPPqqqqPPPPqiiiiiiiif4xPN")
-_SAMPLE = struct.Struct("@PqPPPPPPPPiiiifffi")
+_SAMPLE = struct.Struct("@PqPPPPPPPPiiiifffiPN")
 assert _KV.size == 64
 
 _torch = None
@@ -47,6 +47,10 @@ def _call(fn, *args):
 
 def _stream(index, stream):
     return _raw_stream(index) if stream is None else getattr(stream, "cuda_stream", stream)
+
+
+def _as_stream(stream, index):
+    return stream if isinstance(stream, _torch.cuda.Stream) else _torch.cuda.ExternalStream(_stream(index, stream), index)
 
 
 def _refuse(name, x, dims, index):
@@ -212,8 +216,7 @@ class PagedKV:
                 # torch's allocator orders its reuse by the current stream
                 workspace = table.new_empty((need.value + 3) // 4)
                 if stream is not None:
-                    workspace.record_stream(stream if isinstance(stream, _torch.cuda.Stream)
-                                            else _torch.cuda.ExternalStream(_stream(index, stream), index))
+                    workspace.record_stream(_as_stream(stream, index))
         else:
             _tensor("workspace", workspace, 1, index)
         if workspace is not None:
@@ -271,6 +274,29 @@ def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=N
         token, kept, prob = out
         at = (_vector("token", token, i32, rows, index), _vector("kept", kept, i32, rows, index),
               _vector("prob", prob, f32, rows, index))
-    _call(lib.vx_sample_rows, _SAMPLE.pack(logits.data_ptr(), logits.stride(0), t_at, p_at, m_at, k_at, u_at, *at, rows, n,
-                                           _types[logits.dtype], index, temperature, top_p, min_p, top_k), _stream(index, stream))
+    kind = _types[logits.dtype]
+    space = _sample_space(lib, rows, n, kind, index)
+    work = 0
+    if space:
+        work = logits.new_empty((space + 3) // 4, dtype=i32)
+        if stream is not None:
+            work.record_stream(_as_stream(stream, index))
+        work = work.data_ptr()
+    _call(lib.vx_sample_rows, _SAMPLE.pack(logits.data_ptr(), logits.stride(0), t_at, p_at, m_at, k_at, u_at, *at, rows, n, kind, index,
+                                           temperature, top_p, min_p, top_k, work, space), _stream(index, stream))
     return token, kept, prob
+
+
+_spaces = {}  # (rows, n, type, device) -> bytes of workspace
+
+
+def _sample_space(lib, rows, n, kind, index):
+    key = rows, n, kind, index
+    space = _spaces.get(key)
+    if space is None:
+        need = ctypes.c_size_t()
+        _call(lib.vx_sample_rows_workspace, _SAMPLE.pack(*(0,) * 10, *key, 0, 0, 0, 0, 0, 0), ctypes.byref(need))
+        if len(_spaces) >= 4096:
+            _spaces.clear()
+        space = _spaces[key] = need.value
+    return space
