@@ -75,6 +75,29 @@ def test_flat_rows_and_ties(dtype):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+def test_many_long_rows(dtype):
+    """Rows enough to keep the GPU busy with a block each: ordinary, flat, few
+    distinct values, and one value more than 65536 times."""
+    n, rows, g = 70001, 130, torch.Generator().manual_seed(7)
+    x = torch.randn(rows, n, generator=g) * 2.5
+    x[1::5] *= 0.004
+    x[2::5] = torch.randint(0, 5, (26, n), generator=g).float() * 0.5
+    x[3::5, 1000:] = -1.25
+    x[4::5, 7] = 14.0
+    x[0, 50000:], x[5] = -math.inf, math.nan
+    x[10, ::2] = 0.0
+    x[10, 1::2] = -0.0
+    x = x.to(TYPES[dtype]).to(DEV)
+    r = torch.rand(4, rows, generator=g)
+    t = torch.where(r[0] < 0.15, 0.0, 0.3 + r[0]).tolist()
+    k = torch.where(r[1] < 0.4, 0.0, r[1] * torch.tensor([60.0, 70000.0]).repeat(65)).int().tolist()
+    p = torch.where(r[2] < 0.3, 1.0, 0.3 + 0.699 * r[2]).tolist()
+    m = torch.where(r[3] < 0.5, 0.0, 0.3 * r[3]).tolist()
+    check(x, uniforms(rows, 8), t, k, p, m, most_edges=0.1)
+    check(x[:, 1:], uniforms(rows, 9), 0.9, 0, 0.95, 0.0, most_edges=0.1)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 def test_entries_that_are_not_finite(dtype):
     x = torch.randn(9, 300, generator=torch.Generator().manual_seed(3)) * 2
     x[0] = -math.inf

@@ -222,21 +222,38 @@ inline int check_sample(const char *what, const vx_sample_args *p, SamplePlan *p
   if (!type_ok(p->type)) return batch_fail(VX_E_INVALID, "%s: logits of type %d", what, p->type);
   if (p->rows < 0 || p->n < 1) return batch_fail(VX_E_INVALID, "%s: %d rows of %d logits", what, p->rows, p->n);
   if (p->n > SR_MAXN) return batch_fail(VX_E_RANGE, "%s: %d logits a row, more than %d", what, p->n, SR_MAXN);
-  const int cus = device_cus(p->device);
-  *plan = type_size(p->type) == 4 ? sample_plan<float>(p->rows, p->n, cus) : sample_plan<_Float16>(p->rows, p->n, cus);
+  *plan = sample_plan(p->rows, p->n, device_cus(p->device));
   return VX_OK;
 }
 
+// a launch with S in dynamic LDS; what passes 64 KB is announced once for each device
+template <typename S, void (*K)(SampleArgs)>
+inline int sample_kernel(const char *what, int64_t blocks, const SampleArgs &a, int device, void *stream) {
+  static uint64_t announced = 0;  // bits of devices
+  const uint64_t bit = 1ull << (device & 63);
+  if (sizeof(S) > 64 * 1024 && !(__atomic_load_n(&announced, __ATOMIC_RELAXED) & bit)) {
+    const hipError_t e = hipFuncSetAttribute((const void *)K, hipFuncAttributeMaxDynamicSharedMemorySize, sizeof(S));
+    if (e != hipSuccess) {
+      (void)hipGetLastError();
+      return batch_fail(VX_E_DEVICE, "%s: LDS size rejected: %s", what, hipGetErrorString(e));
+    }
+    __atomic_fetch_or(&announced, bit, __ATOMIC_RELAXED);
+  }
+  return batch_launch(what, K, blocks, SR_NT, sizeof(S), a, stream);
+}
+
 template <typename T>
-inline int sample_launch(const char *what, const SamplePlan &plan, const SampleArgs &a, void *stream) {
-  using H = SrHold<T>;
-  if (!plan.chunks)
-    return batch_launch(what, plan.held ? sample_held_kernel<T, H::U> : sample_rows_kernel<T>, a.rows, SR_NT, 0, a, stream);
+inline int sample_launch(const char *what, const SamplePlan &plan, const SampleArgs &a, int device, void *stream) {
+  if (!plan.chunks) {
+    if (plan.held) return sample_kernel<SrShared, sample_rows_kernel<T, true>>(what, a.rows, a, device, stream);
+    if constexpr (sizeof(T) == 2) return sample_kernel<SrValues, sample_values_kernel<T>>(what, a.rows, a, device, stream);
+    else return sample_kernel<SrShared, sample_rows_kernel<T, false>>(what, a.rows, a, device, stream);
+  }
   const int64_t blocks = (int64_t)a.rows * plan.chunks;
-  int rc = batch_launch(what, sample_range_kernel<T, H::SPLIT_U>, blocks, SR_NT, 0, a, stream);
-  if (!rc) rc = batch_launch(what, sample_bins_kernel<T, H::SPLIT_U>, blocks, SR_NT, 0, a, stream);
-  if (!rc) rc = batch_launch(what, sample_gather_kernel<T, H::SPLIT_U>, blocks, SR_NT, 0, a, stream);
-  if (!rc) rc = batch_launch(what, sample_finish_kernel<T>, a.rows, SR_NT, 0, a, stream);
+  int rc = sample_kernel<SrShared, sample_range_kernel<T>>(what, blocks, a, device, stream);
+  if (!rc) rc = sample_kernel<SrShared, sample_bins_kernel<T>>(what, blocks, a, device, stream);
+  if (!rc) rc = sample_kernel<SrShared, sample_gather_kernel<T>>(what, blocks, a, device, stream);
+  if (!rc) rc = sample_kernel<SrShared, sample_finish_kernel<T>>(what, a.rows, a, device, stream);
   return rc;
 }
 
@@ -259,9 +276,9 @@ inline int sample_rows(const vx_sample_args *p, void *stream) {
                      plan.chunks, plan.chunk, (char *)p->workspace};
   OnDevice on(p->device);
   if (on.status != hipSuccess) return batch_fail(VX_E_DEVICE, "%s: device %d: %s", what, p->device, hipGetErrorString(on.status));
-  return p->type == VX_TYPE_F32 ? sample_launch<float>(what, plan, a, stream)
-         : p->type == VX_TYPE_F16 ? sample_launch<_Float16>(what, plan, a, stream)
-                                  : sample_launch<__bf16>(what, plan, a, stream);
+  return p->type == VX_TYPE_F32 ? sample_launch<float>(what, plan, a, p->device, stream)
+         : p->type == VX_TYPE_F16 ? sample_launch<_Float16>(what, plan, a, p->device, stream)
+                                  : sample_launch<__bf16>(what, plan, a, p->device, stream);
 }
 
 }  // namespace vx

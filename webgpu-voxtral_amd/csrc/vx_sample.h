@@ -45,7 +45,7 @@ struct SampleArgs {
 
 constexpr int SR_NT = 1024, SR_WAVES = SR_NT / 64;
 constexpr int SR_PER = 2;  // bins and gathered entries of a thread
-constexpr int SR_BINS = SR_PER * SR_NT, SR_CELLS = 2 * SR_NT, SR_LIST = SR_PER * SR_NT;
+constexpr int SR_BINS = SR_PER * SR_NT, SR_CELLS = 2048, SR_LIST = SR_PER * SR_NT;
 constexpr int SR_MAXN = 1 << 20;  // 2^43 weights: sums stay below 2^63
 constexpr int SR_FIX = 43;
 constexpr int SR_MAXCHUNKS = 160;
@@ -81,33 +81,46 @@ struct SrBin {
   }
 };
 
-// Running sums are those before a bin, with the total behind the last one.
-struct SrShared {
-  uint64_t mass[SR_BINS + 1];
-  uint32_t count[SR_BINS + 1];
-  uint32_t fill[SR_BINS];  // where a gathered bin's next entry goes; ~0: not gathered
-  union {
-    struct {
-      uint64_t list[SR_LIST], list_w[SR_LIST];
-    };
-    struct {
-      uint64_t cell_mass[SR_CELLS];
-      uint32_t cell_count[SR_CELLS];
-    };
-  };
+// What every form keeps in LDS, and behind it one of the forms' own
+struct SrCommon {
   double tab[32];  // 2^(i / 32)
   uint64_t wave_m[SR_WAVES], found_m, found_e;
   uint32_t wave_c[SR_WAVES], found_c, n_list;
   int found[8];
   float wave_f[SR_WAVES];
 };
+// Running sums are those before a bin, with the total behind the last one.
+struct SrShared : SrCommon {
+  uint64_t mass[SR_BINS + 1];
+  uint32_t count[SR_BINS + 1];
+  uint32_t fill[SR_BINS];  // where a gathered bin's next entry goes; ~0: not gathered
+  union {
+    struct {
+      uint64_t list[SR_LIST], sorted[SR_LIST];
+    };
+    struct {
+      uint64_t cell_mass[SR_CELLS];
+      uint32_t cell_count[SR_CELLS];
+    };
+  };
+};
+// 16-bit logits: how often each value occurs (two to a word, by falling key),
+// and running sums over groups of 64 values
+constexpr int SR_GROUPS = 1024;
+struct SrValues : SrCommon {
+  uint64_t mass[SR_GROUPS + 1];
+  uint32_t count[SR_GROUPS + 1];
+  uint32_t often[1 << 15];
+};
 
 // The block's LDS, always by its own name: a generic pointer to it would make
 // every access a flat one.
-__device__ __forceinline__ SrShared &sr_shared() {
-  __shared__ SrShared s;
-  return s;
+template <typename S>
+__device__ __forceinline__ S &sr_lds() {
+  extern __shared__ __attribute__((aligned(16))) unsigned char sr_smem[];
+  return *(S *)sr_smem;
 }
+__device__ __forceinline__ SrShared &sr_shared() { return sr_lds<SrShared>(); }
 
 // 2^t for t <= 0 to about 10^-11 of itself, as a multiple of 2^-43: t is
 // split into k / 32 and a rest below 1/64, whose power is taken from its
@@ -133,72 +146,95 @@ struct SrWeight {
   }
 };
 
-// Entries of a row: f(index, x) for each that is in the order.  Both kinds
-// read 16 bytes a thread at a time from aligned addresses.
-// Up to U chunks of 16 bytes a thread, kept in registers from the first pass on
-template <typename T, int U>
-struct SrHeld {
-  static constexpr int V = 16 / sizeof(T), MOST = SR_NT * U * V - V + 1;
-  float x[U * V];
-  int at;  // the index of this thread's first one
-  __device__ __forceinline__ void load(const T *row, int from, int to) {
-    const T *p = row + from;
-    const int off = (int)(((uintptr_t)p & 15) / sizeof(T));  // p - off is aligned
-    at = from + (int)threadIdx.x * V - off;
-    PgVec<T, V> v[U];
+// Entries of a row: f(index, x) for each that is in the order.
+// From memory, 16 bytes a thread at a time from aligned addresses; entries
+// from .. to - 1 of the row.  While four such loads are worked on, the next
+// four are on their way: 64 KB a block.  (U 1: a rare path's, for its size.)
+template <typename T, int U = 4>
+struct SrStream {
+  static constexpr int V = 16 / sizeof(T);
+  const T *row;
+  int from, to;
+  // U times a thread's V entries, from i on (i may lie before `from`)
+  __device__ __forceinline__ void load(int i, PgVec<T, V> (&x)[U]) const {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const int i = at + u * SR_NT * V;
+    for (int u = 0; u < U; u++, i += SR_NT * V) {
       if (i >= from && i + V <= to) {
-        v[u] = *(const PgVec<T, V> *)(row + i);
+        x[u] = *(const PgVec<T, V> *)(row + i);
       } else {
 #pragma unroll
-        for (int j = 0; j < V; j++) v[u].x[j] = i + j >= from && i + j < to ? row[i + j] : (T)NAN;
+        for (int j = 0; j < V; j++) x[u].x[j] = i + j >= from && i + j < to ? row[i + j] : (T)NAN;
+      }
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    raw([&](int i, T x) {
+      const float y = (float)x;
+      if (y > -INFINITY) f(i, y);
+    });
+  }
+  // f(index, element), for all (and NaN for some that there are not)
+  template <typename F>
+  __device__ __forceinline__ void raw(F f) const {
+    const int off = (int)(((uintptr_t)(row + from) & 15) / sizeof(T));  // row + from - off is aligned
+    int i = from - off + (int)threadIdx.x * V;
+    PgVec<T, V> x[U], next[U];
+    load(i, x);
+#pragma unroll 1
+    for (;;) {
+      const int then = i + U * SR_NT * V;
+      load(then, next);
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int j = 0; j < V; j++) f(i + u * SR_NT * V + j, x[u].x[j]);
+      if (then >= to) break;
+#pragma unroll
+      for (int u = 0; u < U; u++) x[u] = next[u];
+      i = then;
+    }
+  }
+};
+// Kept in LDS from the first pass on
+constexpr int SR_HOLD = 12288;
+struct SrHeld {
+  int n;
+  static __device__ __forceinline__ float *held() {
+    __shared__ float x[SR_HOLD];
+    return x;
+  }
+  template <typename T>
+  __device__ __forceinline__ void load(const SrStream<T> &from) {
+    constexpr int V = 16 / sizeof(T), U = (SR_HOLD + V - 1 + SR_NT * V - 1) / (SR_NT * V);
+    n = from.to;
+    const int off = (int)(((uintptr_t)from.row & 15) / sizeof(T)), i0 = (int)threadIdx.x * V - off;
+    PgVec<T, V> x[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int i = i0 + u * SR_NT * V;
+      if (i >= 0 && i + V <= n) {
+        x[u] = *(const PgVec<T, V> *)(from.row + i);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; j++) x[u].x[j] = i + j >= 0 && i + j < n ? from.row[i + j] : (T)NAN;
       }
     }
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
-      for (int j = 0; j < V; j++) x[u * V + j] = (float)v[u].x[j];
-  }
-  template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-#pragma unroll
-    for (int u = 0; u < U; u++)
-#pragma unroll
-      for (int j = 0; j < V; j++)
-        if (x[u * V + j] > -INFINITY) f(at + u * SR_NT * V + j, x[u * V + j]);
-  }
-};
-// Any number, read again in every pass
-template <typename T>
-struct SrStream {
-  const T *row;
-  int n;
-  template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-    constexpr int V = 16 / sizeof(T), U = 2;
-    const int off = (int)(((uintptr_t)row & 15) / sizeof(T));
-    const int chunks = (n + off + V - 1) / V;
-    for (int c0 = 0; c0 < chunks; c0 += SR_NT * U) {
-      PgVec<T, V> x[U];
-#pragma unroll
-      for (int u = 0; u < U; u++) {
-        const int i = (c0 + u * SR_NT + (int)threadIdx.x) * V - off;
-        if (i >= 0 && i + V <= n) {
-          x[u] = *(const PgVec<T, V> *)(row + i);
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; j++) x[u].x[j] = i + j >= 0 && i + j < n ? row[i + j] : (T)NAN;
-        }
+      for (int j = 0; j < V; j++) {
+        const int i = i0 + u * SR_NT * V + j;
+        if (i >= 0 && i < n) held()[i] = (float)x[u].x[j];
       }
-#pragma unroll
-      for (int u = 0; u < U; u++)
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-          const float y = (float)x[u].x[j];
-          if (y > -INFINITY) f((c0 + u * SR_NT + (int)threadIdx.x) * V - off + j, y);
-        }
+    __syncthreads();
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += SR_NT) {
+      const float x = held()[i];
+      if (x > -INFINITY) f(i, x);
     }
   }
 };
@@ -303,12 +339,12 @@ __device__ __forceinline__ bool sr_inside(uint64_t target, uint64_t before, uint
   return before < target && target <= after;
 }
 
-// the first entry and the least value over the block
+// The first entry and the least value over the block.  The entry's index is
+// found where it is asked for (a greedy choice), else 0.
 template <typename E>
-__device__ __forceinline__ void sr_range(const E &entries, uint64_t &first, float &least) {
+__device__ __forceinline__ void sr_range(const E &entries, bool index, uint64_t &first, float &least) {
   SrShared &s = sr_shared();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  // the maximum alone is one instruction an entry; its first index is looked for in the wave that has it
   float max = -INFINITY, min = INFINITY;
   entries.each([&](int, float x) {
     max = fmaxf(max, x);
@@ -320,7 +356,7 @@ __device__ __forceinline__ void sr_range(const E &entries, uint64_t &first, floa
     min = fminf(min, __shfl_xor(min, d, 64));
   }
   if (lane == 0) s.wave_f[wave] = min, s.wave_m[wave] = sr_key(max);
-  if (threadIdx.x == 0) s.found_c = ~0u;
+  if (threadIdx.x == 0) s.found_c = index ? ~0u : 0;
   __syncthreads();
   uint32_t key = 0;
   least = INFINITY;
@@ -329,7 +365,7 @@ __device__ __forceinline__ void sr_range(const E &entries, uint64_t &first, floa
     key = s.wave_m[w] > key ? (uint32_t)s.wave_m[w] : key;
     least = fminf(least, s.wave_f[w]);
   }
-  if (key && sr_key(max) == key) {
+  if (index && key && sr_key(max) == key) {  // a wave that has the maximum
     uint32_t at = ~0u;
     entries.each([&](int i, float x) {
       if (sr_key(x) == key) at = (uint32_t)i < at ? (uint32_t)i : at;
@@ -341,7 +377,7 @@ __device__ __forceinline__ void sr_range(const E &entries, uint64_t &first, floa
     }
     if (lane == 0) atomicMin(&s.found_c, at);
   }
-  __syncthreads();
+  if (index) __syncthreads();
   first = key ? sr_entry(key, (int)s.found_c) : ~0ull;
 }
 
@@ -444,35 +480,52 @@ __device__ __forceinline__ uint32_t sr_choose(const SrRow &q, SrCuts &cut) {
   return n;
 }
 
-// A thread's gathered entries and their places: the entries and weights before
-// each
+// A thread's gathered entries, in order, and their places: the entries and
+// weights before each
 struct SrPlaces {
   uint64_t e[SR_PER], w[SR_PER], m[SR_PER];
   uint32_t c[SR_PER];
   int b[SR_PER];  // bins; -1: none
   // Of the list's n entries, those of a bin lie together, at from .. to - 1,
   // running on from the sums (c, m) before it: before(bin, from, to, c, m).
+  // Each is put to its place by the number of those in its bin that come
+  // before it, then their weights are summed.
   template <typename F>
   __device__ __forceinline__ void rank(const SrRow &q, uint32_t n, F before) {
     SrShared &s = sr_shared();
+    uint32_t from, to;
 #pragma unroll
     for (int i = 0; i < SR_PER; i++) {
       const uint32_t at = threadIdx.x + i * SR_NT;
-      e[i] = at < n ? s.list[at] : ~0ull;
+      if (at >= n) continue;
+      const uint64_t x = s.list[at];
+      before(q.bin(sr_value_of(x)), from, to, c[0], m[0]);
+      uint32_t place = from;
+#pragma unroll 8
+      for (uint32_t j = from; j < to; j++) place += s.list[j] < x;
+      s.sorted[place] = x;
+    }
+    __syncthreads();
+    uint64_t sum[SR_PER], total;
+    uint32_t none[SR_PER] = {}, nothing;
+#pragma unroll
+    for (int i = 0; i < SR_PER; i++) {
+      const uint32_t at = threadIdx.x * SR_PER + i;
+      e[i] = at < n ? s.sorted[at] : ~0ull;
       b[i] = at < n ? q.bin(sr_value_of(e[i])) : -1;
       w[i] = at < n ? q.weight(sr_value_of(e[i])) : 0;
-      s.list_w[at] = w[i];
+      sum[i] = w[i];
     }
+    sr_scan(none, sum, nothing, total);
+#pragma unroll
+    for (int i = 0; i < SR_PER; i++) s.list[threadIdx.x * SR_PER + i] = sum[i];  // before each place
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < SR_PER; i++) {
       if (b[i] < 0) continue;
-      uint32_t from, to;
       before(b[i], from, to, c[i], m[i]);
-      for (uint32_t j = from; j < to; j++) {
-        const uint64_t o = s.list[j], ow = s.list_w[j];
-        if (o < e[i]) c[i]++, m[i] += ow;
-      }
+      c[i] += threadIdx.x * SR_PER + i - from;
+      m[i] += sum[i] - s.list[from];
     }
   }
   // f(i) for each entry there is
@@ -686,7 +739,7 @@ __device__ __forceinline__ void sr_row(const E &entries, const S &again, const S
   sr_clear();
   uint64_t first;
   float least;
-  sr_range(entries, first, least);
+  sr_range(entries, !(q.temp > 0), first, least);
   if (sr_simple(q, first, a, r, threadIdx.x == 0)) return;
   q.range(first, least);
   sr_bins(entries, q);
@@ -705,34 +758,271 @@ __device__ __forceinline__ void sr_row(const E &entries, const S &again, const S
     SrSearch<S>{again, q}.finish(cut, a, r);
   }
 }
-template <typename T, int U>
-__global__ __launch_bounds__(SR_NT) void sample_held_kernel(SampleArgs a) {
-  const int r = blockIdx.x;
-  SrHeld<T, U> entries;
-  entries.load((const T *)a.logits + r * a.row_stride, 0, a.n);
-  sr_row(entries, SrStream<T>{(const T *)a.logits + r * a.row_stride, a.n}, a, r);
-}
-template <typename T>
+template <typename T, bool HELD>
 __global__ __launch_bounds__(SR_NT) void sample_rows_kernel(SampleArgs a) {
   const int r = blockIdx.x;
-  const SrStream<T> entries{(const T *)a.logits + r * a.row_stride, a.n};
-  sr_row(entries, entries, a, r);
+  const SrStream<T> stream{(const T *)a.logits + r * a.row_stride, 0, a.n};
+  if constexpr (HELD) {
+    SrHeld held;
+    held.load(stream);
+    sr_row(held, held, a, r);
+  } else {
+    sr_row(stream, SrStream<T, 1>{stream.row, 0, a.n}, a, r);
+  }
+}
+
+// A block a row of 16-bit logits: a pass counts how often each of the 65536
+// values occurs, which is one LDS addition an entry; everything up to the
+// draw then goes by values and their numbers, with one weight a value.  A
+// second pass finds the entry among those of the drawn value.
+// Values by falling key: place 0 is the largest.
+template <typename T>
+__device__ __forceinline__ float sr_place_value(uint32_t place) {
+  const uint32_t key = 0xffffu - place, bits = key & 0x8000u ? key & 0x7fffu : ~key & 0xffffu;
+  const uint16_t b = (uint16_t)bits;
+  return (float)__builtin_bit_cast(T, b);
+}
+// (the second zero counts as the first; ~0: not in the order)
+template <typename T>
+__device__ __forceinline__ uint32_t sr_place(T x) {
+  constexpr uint32_t inf = __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
+  uint32_t b = __builtin_bit_cast(uint16_t, x);
+  b = b == 0x8000u ? 0 : b;
+  return (b & 0x7fffu) > inf || b == (0x8000u | inf) ? ~0u : b & 0x8000u ? b : 0x7fffu - b;
+}
+
+template <typename T>
+struct SrByValue {
+  // a value in its place among the others: entries and weights before it, its
+  // number and weight
+  struct At {
+    uint32_t place, before, number;
+    uint64_t before_m, w;
+  };
+  static __device__ __forceinline__ uint32_t often(uint32_t place) {
+    return sr_lds<SrValues>().often[place >> 1] >> (16 * (place & 1)) & 0xffffu;
+  }
+  // The value at lane l of group `group`, and the sums before it; every wave
+  // does the same.
+  static __device__ __forceinline__ At lane(const SrRow &q, int group) {
+    const SrValues &s = sr_lds<SrValues>();
+    const int l = threadIdx.x & 63;
+    At v;
+    v.place = 64 * group + l;
+    v.number = often(v.place);
+    v.w = v.number ? q.weight(sr_place_value<T>(v.place)) : 0;
+    uint32_t c = v.number;
+    uint64_t m = v.number * v.w;
+    const uint32_t own = c;
+    const uint64_t own_m = m;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t oc = __shfl_up(c, d, 64);
+      const uint64_t om = __shfl_up((unsigned long long)m, d, 64);
+      if (l >= d) c += oc, m += om;
+    }
+    v.before = s.count[group] + c - own;
+    v.before_m = s.mass[group] + m - own_m;
+    return v;
+  }
+  // lane `from`'s value in every lane
+  static __device__ __forceinline__ At of(const At &v, int from) {
+    At r;
+    r.place = __shfl(v.place, from, 64);
+    r.before = __shfl(v.before, from, 64);
+    r.number = __shfl(v.number, from, 64);
+    r.before_m = __shfl((unsigned long long)v.before_m, from, 64);
+    r.w = __shfl((unsigned long long)v.w, from, 64);
+    return r;
+  }
+  // the value that a running count or sum falls on
+  static __device__ __forceinline__ At find(const SrRow &q, bool by_count, uint64_t target) {
+    SrValues &s = sr_lds<SrValues>();
+    const int t = threadIdx.x;
+    __syncthreads();
+    if (by_count ? sr_inside(target, s.count[t], s.count[t + 1]) : sr_inside(target, s.mass[t], s.mass[t + 1])) s.found[0] = t;
+    __syncthreads();
+    const At v = lane(q, s.found[0]);
+    const bool is = by_count ? sr_inside(target, v.before, v.before + v.number) : sr_inside(target, v.before_m, v.before_m + v.number * v.w);
+    return of(v, __ffsll((unsigned long long)__ballot(is)) - 1);
+  }
+  // the number of a value's entries that a sum takes
+  static __device__ __forceinline__ uint32_t part(const At &v, uint64_t target) {
+    return (uint32_t)((target - v.before_m + v.w - 1) / v.w);
+  }
+};
+static_assert(SR_GROUPS == SR_NT, "a group a thread");
+
+template <typename T>
+__global__ __launch_bounds__(SR_NT) void sample_values_kernel(SampleArgs a) {
+  using B = SrByValue<T>;
+  SrValues &s = sr_lds<SrValues>();
+  const int r = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const SrStream<T> stream{(const T *)a.logits + r * a.row_stride, 0, a.n};
+  SrRow q;
+  q.settings(a, r);
+  for (int i = t; i < (1 << 15) / 4; i += SR_NT) ((u32x4 *)s.often)[i] = u32x4{0, 0, 0, 0};
+  if (t < 32) s.tab[t] = exp2(t / 32.0);
+  if (t == 0) s.n_list = 0, s.found_c = 0, s.found[1] = 0x10000;
+  __syncthreads();
+  uint32_t n = 0;
+  stream.raw([&](int, T x) {
+    const uint32_t p = sr_place(x);
+    if (p == ~0u) return;
+    atomicAdd(&s.often[p >> 1], 1u << (16 * (p & 1)));
+    n++;
+  });
+  for (int d = 32; d > 0; d >>= 1) n += __shfl_xor(n, d, 64);
+  if (lane == 0) atomicAdd(&s.n_list, n);
+  __syncthreads();
+
+  // the first value there is; words 1024 i + t are this thread's
+  constexpr int WORDS = (1 << 15) / SR_NT;
+  uint32_t some = 0, sum = 0, first = 0x10000;
+#pragma unroll
+  for (int i = 0; i < WORDS; i++) {
+    const uint32_t w = s.often[i * SR_NT + t];
+    some |= (uint32_t)(w != 0) << i;
+    sum += (w & 0xffffu) + (w >> 16);
+  }
+  if (some) {
+    const int i = __ffs(some) - 1;
+    first = 2 * (i * SR_NT + t) + (s.often[i * SR_NT + t] & 0xffffu ? 0 : 1);
+  }
+  for (int d = 32; d > 0; d >>= 1) {
+    const uint32_t o = __shfl_xor(first, d, 64);
+    first = o < first ? o : first;
+    sum += __shfl_xor(sum, d, 64);
+  }
+  if (lane == 0) {
+    atomicMin(&s.found[1], (int)first);
+    atomicAdd(&s.found_c, sum);
+  }
+  __syncthreads();
+  first = s.found[1];
+  if (s.found_c != s.n_list) {  // a value that occurs 65536 times or more does not fit its half of a word
+    __syncthreads();
+    const SrStream<T, 1> again{stream.row, 0, a.n};
+    sr_row(again, again, a, r);
+    return;
+  }
+  typename B::At v{first, 0, 0, 0, 1};  // the value that is drawn, and which of its entries
+  uint32_t turn = 1, count = 1;
+  uint64_t mass = 1ull << SR_FIX;
+  if (first > 0xffffu) {
+    sr_simple(q, ~0ull, a, r, t == 0);
+    return;
+  }
+  q.range(sr_entry(sr_key(sr_place_value<T>(first)), 0), 0);
+  if (q.temp > 0) {
+    // sums over groups of 64 values: 32 words, half a wave's
+#pragma unroll 1
+    for (int i = 0; i < WORDS; i++) {
+      uint32_t c = 0;
+      uint64_t m = 0;
+      if (__any(some >> i & 1)) {
+        const uint32_t w = s.often[i * SR_NT + t], p = 2 * (i * SR_NT + t);
+        const uint32_t c0 = w & 0xffffu, c1 = w >> 16;
+        c = c0 + c1;
+        if (c0) m = c0 * q.weight(sr_place_value<T>(p));
+        if (c1) m += c1 * q.weight(sr_place_value<T>(p + 1));
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
+          c += __shfl_xor(c, d, 64);
+          m += __shfl_xor((unsigned long long)m, d, 64);
+        }
+      }
+      if ((t & 31) == 0) s.count[i * 32 + (t >> 5)] = c, s.mass[i * 32 + (t >> 5)] = m;
+    }
+    __syncthreads();
+    uint32_t cs[1] = {s.count[t]};
+    uint64_t ms[1] = {s.mass[t]};
+    sr_scan(cs, ms, count, mass);
+    s.count[t] = cs[0];
+    s.mass[t] = ms[0];
+    if (t == 0) s.count[SR_GROUPS] = count, s.mass[SR_GROUPS] = mass;
+    __syncthreads();
+    if (q.top_k > 0 && (uint32_t)q.top_k < count) {
+      v = B::find(q, true, q.top_k);
+      count = q.top_k;
+      mass = v.before_m + (count - v.before) * v.w;
+    }
+    const uint64_t goal = q.goal(mass);
+    if (q.min_p > 0.0f) {
+      // the last place whose value's key is not below min-p's
+      const uint32_t key = q.min_p_key();
+      uint32_t lo = first, hi = 0x10000;  // lo: not below, hi: below
+      while (hi - lo > 1) {
+        const uint32_t by = (hi - lo + 63) / 64, at = lo + by * lane;
+        const bool yes = at < hi && sr_key(sr_place_value<T>(at)) >= key;
+        const int i = 63 - __clzll(__ballot(yes));
+        hi = lo + by * (i + 1) < hi ? lo + by * (i + 1) : hi;
+        lo = lo + by * i;
+      }
+      const typename B::At w = B::of(B::lane(q, lo >> 6), lo & 63);
+      const uint32_t c = w.before + w.number;
+      if (c < count) count = c, mass = w.before_m + w.number * w.w;
+    }
+    if (goal <= mass) {
+      v = B::find(q, false, goal);
+      const uint32_t some_of = B::part(v, goal), c = v.before + some_of;
+      if (c < count) count = c, mass = v.before_m + some_of * v.w;
+    }
+    const uint64_t drawn = q.drawn(mass);
+    v = B::find(q, false, drawn);
+    turn = B::part(v, drawn);
+  }
+
+  // the turn-th entry of the drawn value: counted in 1024 runs of the row
+  __syncthreads();
+  s.often[t] = 0;
+  __syncthreads();
+  int shift = 0;
+  while (((a.n - 1) >> shift) >= SR_NT) shift++;
+  stream.raw([&](int i, T x) {
+    if (sr_place(x) == v.place) atomicAdd(&s.often[i >> shift], 1u);
+  });
+  __syncthreads();
+  uint32_t cs[1] = {s.often[t]}, total;
+  const uint32_t own = cs[0];
+  uint64_t none[1] = {0}, nothing;
+  sr_scan(cs, none, total, nothing);
+  if (sr_inside(turn, cs[0], cs[0] + own)) s.found[0] = t, s.found[1] = turn - cs[0];
+  __syncthreads();
+  if (wave) return;
+  int left = s.found[1];
+  const int from = s.found[0] << shift, to = min(a.n, from + (1 << shift));
+  for (int i = from; i < to; i += 64) {
+    const bool is = i + lane < to && sr_place(stream.row[i + lane]) == v.place;
+    const uint64_t m = __ballot(is);
+    const int here = __popcll(m);
+    if (left > here) {
+      left -= here;
+      continue;
+    }
+    if (is && __popcll(m & ((1ull << lane) - 1)) == left - 1) {
+      a.token[r] = i + lane;
+      if (a.kept) a.kept[r] = (int)count;
+      if (a.prob)
+        a.prob[r] = !(q.temp > 0) ? 1.0f : (float)((q.weight.inf ? 0x1p43 : q.weight.power(sr_place_value<T>(v.place))) / (double)mass);
+    }
+    break;
+  }
 }
 
 // Several blocks a row, for a few long rows: the same passes as launches of
 // their own, sums and gathered entries joined in memory (integers: the order
 // of the blocks does not matter).
 // the range of a chunk's values; clears what the next passes add to
-template <typename T, int U>
+template <typename T>
 __global__ __launch_bounds__(SR_NT) void sample_range_kernel(SampleArgs a) {
   const int r = blockIdx.x / a.chunks, k = blockIdx.x - r * a.chunks;
   SrSplit &g = ((SrSplit *)a.split)[r];
-  SrHeld<T, U> entries;
-  entries.load((const T *)a.logits + r * a.row_stride, k * a.chunk, min(a.n, (k + 1) * a.chunk));
+  const SrStream<T> entries{(const T *)a.logits + r * a.row_stride, k * a.chunk, min(a.n, (k + 1) * a.chunk)};
   for (int i = k * SR_NT + threadIdx.x; i < SR_BINS; i += a.chunks * SR_NT) g.mass[i] = 0, g.count[i] = 0, g.fill[i] = 0;
   uint64_t first;
   float least;
-  sr_range(entries, first, least);
+  sr_range(entries, !((a.temperature ? a.temperature[r] : a.temperature0) > 0), first, least);
   if (threadIdx.x == 0) g.first[k] = first, g.least[k] = least;
 }
 // the row's range from its chunks'
@@ -751,13 +1041,12 @@ __device__ __forceinline__ void sr_joined(const SrSplit &g, int chunks, uint64_t
     least = fminf(least, __shfl_xor(least, d, 64));
   }
 }
-template <typename T, int U>
+template <typename T>
 __global__ __launch_bounds__(SR_NT) void sample_bins_kernel(SampleArgs a) {
   SrShared &s = sr_shared();
   const int r = blockIdx.x / a.chunks, k = blockIdx.x - r * a.chunks, t = threadIdx.x;
   SrSplit &g = ((SrSplit *)a.split)[r];
-  SrHeld<T, U> entries;
-  entries.load((const T *)a.logits + r * a.row_stride, k * a.chunk, min(a.n, (k + 1) * a.chunk));
+  const SrStream<T> entries{(const T *)a.logits + r * a.row_stride, k * a.chunk, min(a.n, (k + 1) * a.chunk)};
   SrRow q;
   q.settings(a, r);
   sr_clear();
@@ -775,13 +1064,12 @@ __global__ __launch_bounds__(SR_NT) void sample_bins_kernel(SampleArgs a) {
       if (s.mass[b]) atomicAdd((unsigned long long *)&g.mass[b], (unsigned long long)s.mass[b]);
     }
 }
-template <typename T, int U>
+template <typename T>
 __global__ __launch_bounds__(SR_NT) void sample_gather_kernel(SampleArgs a) {
   SrShared &s = sr_shared();
   const int r = blockIdx.x / a.chunks, k = blockIdx.x - r * a.chunks, t = threadIdx.x;
   SrSplit &g = ((SrSplit *)a.split)[r];
-  SrHeld<T, U> entries;
-  entries.load((const T *)a.logits + r * a.row_stride, k * a.chunk, min(a.n, (k + 1) * a.chunk));
+  const SrStream<T> entries{(const T *)a.logits + r * a.row_stride, k * a.chunk, min(a.n, (k + 1) * a.chunk)};
   uint32_t c[SR_PER];
   uint64_t m[SR_PER];
 #pragma unroll
@@ -832,35 +1120,30 @@ __global__ __launch_bounds__(SR_NT) void sample_finish_kernel(SampleArgs a) {
     __syncthreads();
     sr_finish(q, cut, n, a, r);
   } else {
-    const SrStream<T> entries{(const T *)a.logits + r * a.row_stride, a.n};
-    SrSearch<SrStream<T>>{entries, q}.finish(cut, a, r);
+    const SrStream<T, 1> entries{(const T *)a.logits + r * a.row_stride, 0, a.n};
+    SrSearch<SrStream<T, 1>>{entries, q}.finish(cut, a, r);
   }
 }
 
-// How rows of n are dealt out: to a block each, held in its registers where
-// they fit, or several blocks each where there are fewer rows than compute
-// units to keep busy
+// How rows of n are dealt out: to a block each, held in its LDS where they
+// fit, or several blocks each where there are fewer rows than compute units to
+// keep busy
 struct SamplePlan {
   int chunks, chunk;  // 0: one block
   bool held;
   size_t bytes;  // of workspace
 };
-template <typename T>
-struct SrHold {
-  static constexpr int U = sizeof(T) == 4 ? 3 : 2, SPLIT_U = sizeof(T) == 4 ? 2 : 1;  // 12288 or 16384 entries; 8192
-};
-template <typename T>
 inline SamplePlan sample_plan(int rows, int n, int cus) {
+  constexpr int most = 8192;
+  static_assert(most * SR_MAXCHUNKS >= SR_MAXN, "chunks");
   SamplePlan p{};
-  p.held = n <= SrHeld<T, SrHold<T>::U>::MOST;
+  p.held = n <= SR_HOLD;
   if (!p.held && rows * 2 <= cus) {
-    const int most = SrHeld<T, SrHold<T>::SPLIT_U>::MOST / 8 * 8;
     p.chunks = (n + most - 1) / most;
     p.chunk = ((n + p.chunks - 1) / p.chunks + 7) / 8 * 8;
     p.bytes = sizeof(SrSplit) * (size_t)rows;
   }
   return p;
 }
-static_assert(SrHeld<float, 2>::MOST / 8 * 8 * SR_MAXCHUNKS >= SR_MAXN && SrHeld<_Float16, 1>::MOST / 8 * 8 * SR_MAXCHUNKS >= SR_MAXN, "chunks");
 
 }  // namespace vx
