@@ -104,8 +104,8 @@ struct SrShared : SrCommon {
     };
   };
 };
-// 16-bit logits: how often each value occurs (two to a word, by falling key),
-// and running sums over groups of 64 values
+// 16-bit logits: how often each value occurs (two to a word, by bit pattern),
+// and running sums over groups of 64 values, by falling value
 constexpr int SR_GROUPS = 1024;
 struct SrValues : SrCommon {
   uint64_t mass[SR_GROUPS + 1];
@@ -146,6 +146,30 @@ struct SrWeight {
   }
 };
 
+// loads that are known to be from device memory: through a generic pointer
+// they would wait for LDS too
+template <typename W>
+__device__ __forceinline__ W sr_global(const void *p) {
+  return *(const __attribute__((address_space(1))) W *)p;
+}
+template <typename T>
+__device__ __forceinline__ T sr_element(const T *p) {
+  if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, sr_global<uint32_t>(p));
+  else return __builtin_bit_cast(T, sr_global<uint16_t>(p));
+}
+// 16 bytes of elements from i on, NaN in place of those outside from .. to - 1
+template <typename T, int V = 16 / sizeof(T)>
+__device__ __forceinline__ PgVec<T, V> sr_elements(const T *row, int i, int from, int to) {
+  PgVec<T, V> x;
+  if (i >= from && i + V <= to) {
+    x = __builtin_bit_cast(PgVec<T, V>, sr_global<u32x4>(row + i));
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; j++) x.x[j] = i + j >= from && i + j < to ? sr_element(row + i + j) : (T)NAN;
+  }
+  return x;
+}
+
 // Entries of a row: f(index, x) for each that is in the order.
 // From memory, 16 bytes a thread at a time from aligned addresses; entries
 // from .. to - 1 of the row.  While four such loads are worked on, the next
@@ -158,25 +182,22 @@ struct SrStream {
   // U times a thread's V entries, from i on (i may lie before `from`)
   __device__ __forceinline__ void load(int i, PgVec<T, V> (&x)[U]) const {
 #pragma unroll
-    for (int u = 0; u < U; u++, i += SR_NT * V) {
-      if (i >= from && i + V <= to) {
-        x[u] = *(const PgVec<T, V> *)(row + i);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; j++) x[u].x[j] = i + j >= from && i + j < to ? row[i + j] : (T)NAN;
-      }
-    }
+    for (int u = 0; u < U; u++, i += SR_NT * V) x[u] = sr_elements(row, i, from, to);
   }
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-    raw([&](int i, T x) {
-      const float y = (float)x;
-      if (y > -INFINITY) f(i, y);
+    vectors([&](int i, const PgVec<T, V> &x) {
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        const float y = (float)x.x[j];
+        if (y > -INFINITY) f(i + j, y);
+      }
     });
   }
-  // f(index, element), for all (and NaN for some that there are not)
+  // f(index, V elements), NaN where there is none; U SR_NT V elements a step
   template <typename F>
-  __device__ __forceinline__ void raw(F f) const {
+  __device__ __forceinline__ int vectors(F f) const {
+    int steps = 0;
     const int off = (int)(((uintptr_t)(row + from) & 15) / sizeof(T));  // row + from - off is aligned
     int i = from - off + (int)threadIdx.x * V;
     PgVec<T, V> x[U], next[U];
@@ -186,14 +207,14 @@ struct SrStream {
       const int then = i + U * SR_NT * V;
       load(then, next);
 #pragma unroll
-      for (int u = 0; u < U; u++)
-#pragma unroll
-        for (int j = 0; j < V; j++) f(i + u * SR_NT * V + j, x[u].x[j]);
-      if (then >= to) break;
+      for (int u = 0; u < U; u++) f(i + u * SR_NT * V, x[u]);
+      steps++;
+      if (then - (int)threadIdx.x * V >= to) break;  // the same for all threads
 #pragma unroll
       for (int u = 0; u < U; u++) x[u] = next[u];
       i = then;
     }
+    return steps;
   }
 };
 // Kept in LDS from the first pass on
@@ -211,15 +232,7 @@ struct SrHeld {
     const int off = (int)(((uintptr_t)from.row & 15) / sizeof(T)), i0 = (int)threadIdx.x * V - off;
     PgVec<T, V> x[U];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const int i = i0 + u * SR_NT * V;
-      if (i >= 0 && i + V <= n) {
-        x[u] = *(const PgVec<T, V> *)(from.row + i);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; j++) x[u].x[j] = i + j >= 0 && i + j < n ? from.row[i + j] : (T)NAN;
-      }
-    }
+    for (int u = 0; u < U; u++) x[u] = sr_elements(from.row, i0 + u * SR_NT * V, 0, n);
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
@@ -775,20 +788,11 @@ __global__ __launch_bounds__(SR_NT) void sample_rows_kernel(SampleArgs a) {
 // values occurs, which is one LDS addition an entry; everything up to the
 // draw then goes by values and their numbers, with one weight a value.  A
 // second pass finds the entry among those of the drawn value.
-// Values by falling key: place 0 is the largest.
+// Values by falling order: the bit pattern at a place (0: the largest).
+__device__ __forceinline__ uint32_t sr_place_bits(uint32_t place) { return place < 0x8000u ? 0x7fffu - place : place; }
 template <typename T>
 __device__ __forceinline__ float sr_place_value(uint32_t place) {
-  const uint32_t key = 0xffffu - place, bits = key & 0x8000u ? key & 0x7fffu : ~key & 0xffffu;
-  const uint16_t b = (uint16_t)bits;
-  return (float)__builtin_bit_cast(T, b);
-}
-// (the second zero counts as the first; ~0: not in the order)
-template <typename T>
-__device__ __forceinline__ uint32_t sr_place(T x) {
-  constexpr uint32_t inf = __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
-  uint32_t b = __builtin_bit_cast(uint16_t, x);
-  b = b == 0x8000u ? 0 : b;
-  return (b & 0x7fffu) > inf || b == (0x8000u | inf) ? ~0u : b & 0x8000u ? b : 0x7fffu - b;
+  return (float)__builtin_bit_cast(T, (uint16_t)sr_place_bits(place));
 }
 
 template <typename T>
@@ -800,7 +804,8 @@ struct SrByValue {
     uint64_t before_m, w;
   };
   static __device__ __forceinline__ uint32_t often(uint32_t place) {
-    return sr_lds<SrValues>().often[place >> 1] >> (16 * (place & 1)) & 0xffffu;
+    const uint32_t bits = sr_place_bits(place);
+    return sr_lds<SrValues>().often[bits >> 1] >> (16 * (bits & 1)) & 0xffffu;
   }
   // The value at lane l of group `group`, and the sums before it; every wave
   // does the same.
@@ -863,29 +868,44 @@ __global__ __launch_bounds__(SR_NT) void sample_values_kernel(SampleArgs a) {
   q.settings(a, r);
   for (int i = t; i < (1 << 15) / 4; i += SR_NT) ((u32x4 *)s.often)[i] = u32x4{0, 0, 0, 0};
   if (t < 32) s.tab[t] = exp2(t / 32.0);
-  if (t == 0) s.n_list = 0, s.found_c = 0, s.found[1] = 0x10000;
+  if (t == 0) s.found_c = 0, s.found[1] = 0x10000;
   __syncthreads();
-  uint32_t n = 0;
-  stream.raw([&](int, T x) {
-    const uint32_t p = sr_place(x);
-    if (p == ~0u) return;
-    atomicAdd(&s.often[p >> 1], 1u << (16 * (p & 1)));
-    n++;
+  const uint32_t n = SrStream<T>::V * 4 * SR_NT * stream.vectors([&](int, const PgVec<T, SrStream<T>::V> &x) {
+#pragma unroll
+    for (int j = 0; j < SrStream<T>::V; j++) {
+      const uint32_t b = __builtin_bit_cast(uint16_t, x.x[j]);
+      atomicAdd(&s.often[b >> 1], b & 1 ? 0x10000u : 1u);
+    }
   });
-  for (int d = 32; d > 0; d >>= 1) n += __shfl_xor(n, d, 64);
-  if (lane == 0) atomicAdd(&s.n_list, n);
   __syncthreads();
 
-  // the first value there is; words 1024 i + t are this thread's
+  // Words 1024 i + t are this thread's: the positive values' for i < 16, the
+  // negative ones' behind them.  What is not in the order is taken out, the
+  // second zero is counted as the first, and the first value there is found.
   constexpr int WORDS = (1 << 15) / SR_NT;
+  constexpr uint32_t inf = __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
   uint32_t some = 0, sum = 0, first = 0x10000;
-#pragma unroll
+#pragma unroll 8
   for (int i = 0; i < WORDS; i++) {
-    const uint32_t w = s.often[i * SR_NT + t];
-    some |= (uint32_t)(w != 0) << i;
+    const uint32_t at = i * SR_NT + t, all = s.often[at];
+    uint32_t w = all;
     sum += (w & 0xffffu) + (w >> 16);
+    if ((at > inf >> 1 && at < 0x4000u) || at >= (0x8000u | inf) >> 1) w = 0;  // NaN, -inf
+    if (at == inf >> 1) w &= 0xffffu;                                          // +inf, and a NaN
+    if (w != all) s.often[at] = w;
+    some |= (uint32_t)(w != 0) << i;
   }
-  if (some) {
+  if (t == 0) {
+    const uint32_t zeros = (s.often[0] & 0xffffu) + (s.often[0x4000] & 0xffffu);
+    if (zeros > 0xffffu) sum++;  // does not fit
+    s.often[0] = (s.often[0] & 0xffff0000u) | (zeros & 0xffffu);
+    s.often[0x4000] &= 0xffff0000u;
+    some = (some & ~0x10001u) | (s.often[0] != 0) | (uint32_t)(s.often[0x4000] != 0) << 16;
+  }
+  if (some & 0xffffu) {
+    const int i = 31 - __clz(some & 0xffffu);
+    first = 0x7fffu - (2 * (i * SR_NT + t) + (s.often[i * SR_NT + t] >> 16 ? 1 : 0));
+  } else if (some) {
     const int i = __ffs(some) - 1;
     first = 2 * (i * SR_NT + t) + (s.often[i * SR_NT + t] & 0xffffu ? 0 : 1);
   }
@@ -900,7 +920,7 @@ __global__ __launch_bounds__(SR_NT) void sample_values_kernel(SampleArgs a) {
   }
   __syncthreads();
   first = s.found[1];
-  if (s.found_c != s.n_list) {  // a value that occurs 65536 times or more does not fit its half of a word
+  if (s.found_c != n) {  // a value that occurs 65536 times or more does not fit its half of a word
     __syncthreads();
     const SrStream<T, 1> again{stream.row, 0, a.n};
     sr_row(again, again, a, r);
@@ -916,23 +936,24 @@ __global__ __launch_bounds__(SR_NT) void sample_values_kernel(SampleArgs a) {
   q.range(sr_entry(sr_key(sr_place_value<T>(first)), 0), 0);
   if (q.temp > 0) {
     // sums over groups of 64 values: 32 words, half a wave's
+    const auto group = [&](int i) { return i < WORDS / 2 ? SR_GROUPS / 2 - 1 - (i * 32 + (t >> 5)) : i * 32 + (t >> 5); };
 #pragma unroll 1
     for (int i = 0; i < WORDS; i++) {
       uint32_t c = 0;
       uint64_t m = 0;
       if (__any(some >> i & 1)) {
-        const uint32_t w = s.often[i * SR_NT + t], p = 2 * (i * SR_NT + t);
+        const uint32_t w = s.often[i * SR_NT + t], b = 2 * (i * SR_NT + t);
         const uint32_t c0 = w & 0xffffu, c1 = w >> 16;
         c = c0 + c1;
-        if (c0) m = c0 * q.weight(sr_place_value<T>(p));
-        if (c1) m += c1 * q.weight(sr_place_value<T>(p + 1));
+        if (c0) m = c0 * q.weight((float)__builtin_bit_cast(T, (uint16_t)b));
+        if (c1) m += c1 * q.weight((float)__builtin_bit_cast(T, (uint16_t)(b + 1)));
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) {
           c += __shfl_xor(c, d, 64);
           m += __shfl_xor((unsigned long long)m, d, 64);
         }
       }
-      if ((t & 31) == 0) s.count[i * 32 + (t >> 5)] = c, s.mass[i * 32 + (t >> 5)] = m;
+      if ((t & 31) == 0) s.count[group(i)] = c, s.mass[group(i)] = m;
     }
     __syncthreads();
     uint32_t cs[1] = {s.count[t]};
@@ -979,8 +1000,25 @@ __global__ __launch_bounds__(SR_NT) void sample_values_kernel(SampleArgs a) {
   __syncthreads();
   int shift = 0;
   while (((a.n - 1) >> shift) >= SR_NT) shift++;
-  stream.raw([&](int i, T x) {
-    if (sr_place(x) == v.place) atomicAdd(&s.often[i >> shift], 1u);
+  const uint32_t bits = sr_place_bits(v.place);
+  const auto is_it = [&](T x) {
+    const uint32_t b = __builtin_bit_cast(uint16_t, x);
+    return b == bits || (bits == 0 && b == 0x8000u);
+  };
+  const uint32_t pair = bits * 0x10001u, sign = bits ? 0 : 0x80008000u;
+  stream.vectors([&](int i, const PgVec<T, SrStream<T>::V> &x) {
+    // a half word of zeros in any of the differences (or a false alarm)
+    uint32_t any = 0;
+#pragma unroll
+    for (int j = 0; j < SrStream<T>::V; j += 2) {
+      const uint32_t w = __builtin_bit_cast(uint16_t, x.x[j]) | (uint32_t)__builtin_bit_cast(uint16_t, x.x[j + 1]) << 16;
+      const uint32_t d = (w ^ pair) & ~sign;
+      any |= (d - 0x00010001u) & ~d;
+    }
+    if (!(any & 0x80008000u)) return;
+#pragma unroll
+    for (int j = 0; j < SrStream<T>::V; j++)
+      if (is_it(x.x[j])) atomicAdd(&s.often[(i + j) >> shift], 1u);
   });
   __syncthreads();
   uint32_t cs[1] = {s.often[t]}, total;
@@ -993,7 +1031,7 @@ __global__ __launch_bounds__(SR_NT) void sample_values_kernel(SampleArgs a) {
   int left = s.found[1];
   const int from = s.found[0] << shift, to = min(a.n, from + (1 << shift));
   for (int i = from; i < to; i += 64) {
-    const bool is = i + lane < to && sr_place(stream.row[i + lane]) == v.place;
+    const bool is = i + lane < to && is_it(sr_element(stream.row + i + lane));
     const uint64_t m = __ballot(is);
     const int here = __popcll(m);
     if (left > here) {
