@@ -252,6 +252,28 @@ struct SrHeld {
   }
 };
 
+// The sums of (c, m) over the lanes up to this one, by DPP: four shifts inside
+// rows of 16 lanes, then the rows' totals handed on (a shift brings 0 where
+// there is no lane).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t sr_dpp(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ void sr_add_dpp(uint32_t &c, uint64_t &m) {
+  const uint64_t o = (uint64_t)sr_dpp<CTRL, ROWS>((uint32_t)(m >> 32)) << 32 | sr_dpp<CTRL, ROWS>((uint32_t)m);
+  c += sr_dpp<CTRL, ROWS>(c);
+  m += o;
+}
+__device__ __forceinline__ void sr_wave_scan(uint32_t &c, uint64_t &m) {
+  sr_add_dpp<0x111, 0xF>(c, m);  // row_shr 1, 2, 4, 8
+  sr_add_dpp<0x112, 0xF>(c, m);
+  sr_add_dpp<0x114, 0xF>(c, m);
+  sr_add_dpp<0x118, 0xF>(c, m);
+  sr_add_dpp<0x142, 0xA>(c, m);  // the last lane of rows 0 and 2 to rows 1 and 3
+  sr_add_dpp<0x143, 0xC>(c, m);  // lane 31 to rows 2 and 3
+}
+
 // the sums of (count, mass) before each of PER items a thread, in thread
 // order, in place; the totals over the block go to (tc, tm)
 template <int PER>
@@ -271,18 +293,13 @@ __device__ __forceinline__ void sr_scan(uint32_t (&c)[PER], uint64_t (&m)[PER], 
   }
   uint32_t ic = ac;
   uint64_t im = am;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t oc = __shfl_up(ic, d, 64);
-    const uint64_t om = __shfl_up((unsigned long long)im, d, 64);
-    if (lane >= d) ic += oc, im += om;
-  }
+  sr_wave_scan(ic, im);
   __syncthreads();
   if (lane == 63) s.wave_c[wave] = ic, s.wave_m[wave] = im;
   __syncthreads();
   tc = 0;
   tm = 0;
-#pragma unroll
+#pragma unroll 4
   for (int w = 0; w < SR_WAVES; w++) {
     if (w == wave) bc = tc, bm = tm;
     tc += s.wave_c[w];
@@ -820,12 +837,7 @@ struct SrByValue {
     uint64_t m = v.number * v.w;
     const uint32_t own = c;
     const uint64_t own_m = m;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t oc = __shfl_up(c, d, 64);
-      const uint64_t om = __shfl_up((unsigned long long)m, d, 64);
-      if (l >= d) c += oc, m += om;
-    }
+    sr_wave_scan(c, m);
     v.before = s.count[group] + c - own;
     v.before_m = s.mass[group] + m - own_m;
     return v;
@@ -885,7 +897,7 @@ __global__ __launch_bounds__(SR_NT) void sample_values_kernel(SampleArgs a) {
   constexpr int WORDS = (1 << 15) / SR_NT;
   constexpr uint32_t inf = __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
   uint32_t some = 0, sum = 0, first = 0x10000;
-#pragma unroll 8
+#pragma unroll 4
   for (int i = 0; i < WORDS; i++) {
     const uint32_t at = i * SR_NT + t, all = s.often[at];
     uint32_t w = all;
