@@ -97,7 +97,7 @@ inline int paged_append(const vx_append_args *p, void *stream) {
   const char *what = "vx_paged_append";
   if (!p) return batch_fail(VX_E_INVALID, "%s: NULL arguments", what);
   AppendArgs a;
-  if (int rc = check_kv(what, p->kv, &a.kv)) return rc;
+  if (int rc = check_kv(what, p->kv, &a.rows.kv)) return rc;
   if (!types_ok(p->type, p->kv.type)) return batch_fail(VX_E_INVALID, "%s: rows of type %d for a cache of type %d", what, p->type, p->kv.type);
   if (p->n_tokens < 0 || p->n_seqs < 0 || p->table_width < 0 || p->n_heads < 0 || p->n_heads > 4096)
     return batch_fail(VX_E_INVALID, "%s: %d tokens, %d sequences, %d table columns, %d heads", what, p->n_tokens, p->n_seqs, p->table_width, p->n_heads);
@@ -114,12 +114,14 @@ inline int paged_append(const vx_append_args *p, void *stream) {
       (p->q && (!aligned16(p->q, es, p->q_row, p->q_head) || !aligned16(p->q_out, es, p->o_row, p->o_head))))
     return batch_fail(VX_E_INVALID, "%s: rows and their strides must be multiples of 16 bytes", what);
   if (p->n_seqs == 0 || p->table_width == 0) return VX_OK;  // no place to write to
-  a.k = p->k, a.v = p->v, a.q = p->n_heads ? p->q : nullptr, a.q_out = p->q_out;
-  a.k_row = p->k_row, a.k_head = p->k_head, a.v_row = p->v_row, a.v_head = p->v_head;
-  a.q_row = p->q_row, a.q_head = p->q_head, a.o_row = p->o_row, a.o_head = p->o_head;
+  AppendRows &r = a.rows;
+  r.k = p->k, r.v = p->v, r.q = p->n_heads ? p->q : nullptr, r.q_out = p->q_out;
+  r.k_row = p->k_row, r.k_head = p->k_head, r.v_row = p->v_row, r.v_head = p->v_head;
+  r.q_row = p->q_row, r.q_head = p->q_head, r.o_row = p->o_row, r.o_head = p->o_head;
+  r.rotary_dim = p->rotary_dim, r.interleaved = p->interleaved;
   a.pos = p->pos, a.seq = p->seq, a.table = p->table, a.table_stride = p->table_stride;
   a.table_width = p->table_width, a.base = p->base, a.n_tokens = p->n_tokens, a.n_seqs = p->n_seqs;
-  a.n_heads = p->n_heads, a.head_dim = p->kv.head_dim, a.rotary_dim = p->rotary_dim, a.interleaved = p->interleaved;
+  a.n_heads = p->n_heads, a.head_dim = p->kv.head_dim;
   // theta^(-2 i / rotary_dim) as a product of two of 16 powers
   const double step = p->rotary_dim ? -2.0 * std::log2(p->theta) / p->rotary_dim : 0;
   double low[8];
@@ -130,8 +132,8 @@ inline int paged_append(const vx_append_args *p, void *stream) {
   }
   OnDevice on(p->kv.device);
   if (on.status != hipSuccess) return batch_fail(VX_E_DEVICE, "%s: device %d: %s", what, p->kv.device, hipGetErrorString(on.status));
-  return with_types(p->type, p->kv.type, [&](auto r, auto c) {
-    return batch_launch(what, paged_append_kernel<decltype(r), decltype(c)>, a.n_tokens, PA_NT, 0, a, stream);
+  return with_types(p->type, p->kv.type, [&](auto rt, auto ct) {
+    return batch_launch(what, paged_append_kernel<decltype(rt), decltype(ct)>, a.n_tokens, PA_NT, 0, a, stream);
   });
 }
 

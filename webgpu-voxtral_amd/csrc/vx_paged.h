@@ -59,6 +59,24 @@ __device__ __forceinline__ void pg_load(const T *p, float (&y)[N]) {
     for (int j = 0; j < C; j++) y[i + j] = pg_f32(v.x[j]);
   }
 }
+// eight elements at p, aligned to 16 bytes, as they are, and as f32
+template <typename T>
+struct PgEight {
+  static constexpr int W = sizeof(T) / 2, C = 16 / sizeof(T);
+  u32x4 w[W];
+  __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+    for (int i = 0; i < W; i++) w[i] = *(const u32x4 *)(p + i * C);
+  }
+  __device__ __forceinline__ void get(float (&y)[8]) const {
+#pragma unroll
+    for (int i = 0; i < W; i++) {
+      const PgVec<T, C> v = __builtin_bit_cast(PgVec<T, C>, w[i]);
+#pragma unroll
+      for (int j = 0; j < C; j++) y[i * C + j] = (float)v.x[j];
+    }
+  }
+};
 template <typename T, int N>
 __device__ __forceinline__ void pg_store(T *p, const float (&y)[N]) {
   constexpr int C = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
@@ -75,15 +93,18 @@ __device__ __forceinline__ void pg_store(T *p, const float (&y)[N]) {
 // Token t, position p = pos[t]: every head's pair i of the first rotary_dim
 // elements turns by p theta^(-2 i / rotary_dim); K (turned) and V go to slot
 // p - base of sequence seq[t], Q (turned) to q_out.
-struct AppendArgs {
+struct AppendRows {
   PagedKV kv;
   const void *k, *v, *q;
   void *q_out;
   int64_t k_row, k_head, v_row, v_head, q_row, q_head, o_row, o_head;
+  int rotary_dim, interleaved;
+};
+struct AppendArgs {
+  AppendRows rows;
   const int *pos, *seq, *table;
   int64_t table_stride;
   int table_width, base, n_tokens, n_seqs, n_heads, head_dim;
-  int rotary_dim, interleaved;
   // revolutions a position for each pair: theta^(-2 i / rotary_dim) / (2 pi).
   // In 64 bits: at position 10^6 an f32 frequency is off by 0.06 radians.
   double turns[64];
@@ -93,76 +114,93 @@ constexpr int PA_NT = 256;
 
 // One block a token: its 64 angles are reduced to a revolution in 64 bits and
 // their sine and cosine taken once, then shared by every head through LDS.
-// A thread moves two chunks of 8 elements: neighbours, or the two halves of a
-// pair when pairs are (i, i + rotary_dim / 2).
-template <typename RT, typename CT>
-__global__ __launch_bounds__(PA_NT) void paged_append_kernel(AppendArgs a) {
-  __shared__ float cs[64], sn[64];
-  const int t = blockIdx.x, tid = threadIdx.x;
-  const int p = a.pos[t], s = a.seq ? a.seq[t] : t;
-  if (p < 0 || s < 0 || s >= a.n_seqs) return;
-  const int64_t slot = (int64_t)p - a.base;
-  const int page = pg_page(a.table + (int64_t)s * a.table_stride, a.table_width, slot, a.kv.page_shift, a.kv.n_pages);
-  if (page < 0) return;
-  const int half = a.rotary_dim >> 1;
-  if (tid < half) {
-    const double r = p * a.turns[tid];
-    sincospif(2.0f * (float)(r - rint(r)), &sn[tid], &cs[tid]);
-  }
-  __syncthreads();
-  const int per = a.head_dim >> 4, hkv = a.kv.n_kv_heads;
-  const int heads = 2 * hkv + (a.q ? a.n_heads : 0);
-  const int64_t at = page * a.kv.page_stride + (slot & (a.kv.page_size - 1)) * a.kv.token_stride;
-  for (int w = tid; w < heads * per; w += PA_NT) {
-    const int h = w / per, c = w - h * per;
-    // elements d0.. and d1.. of the head, and the first pair they hold
-    const bool turned = c < (a.rotary_dim >> 4);
-    int d0 = 16 * c, d1 = d0 + 8;
-    if (turned && !a.interleaved) d0 = 8 * c, d1 = d0 + half;
-    float x[8], y[8];
-    if (h >= hkv && h < 2 * hkv) {
-      const RT *src = (const RT *)a.v + t * a.v_row + (h - hkv) * a.v_head;
-      CT *dst = (CT *)a.kv.v + at + (h - hkv) * a.kv.head_stride;
-      pg_load(src + d0, x);
-      pg_load(src + d1, y);
-      pg_store(dst + d0, x);
-      pg_store(dst + d1, y);
-      continue;
-    }
+// A thread moves chunks of 16 elements, two at a time: neighbouring eights, or
+// those of the two halves of a pair when pairs are (i, i + rotary_dim / 2).
+// Bound by memory where there are many tokens, by latency where there are few:
+// the first two chunks are asked for before the token's page and angles are
+// known.
+template <typename RT>
+struct PaChunk {
+  int h, c, d0, d1;  // head (keys, values, queries), chunk, its elements' places
+  bool turned;
+  PgEight<RT> x, y;
+  __device__ __forceinline__ void load(const AppendRows &a, int t, int w, int per) {
+    const int hkv = a.kv.n_kv_heads;
+    h = w / per;
+    c = w - h * per;
     const RT *src = h < hkv ? (const RT *)a.k + t * a.k_row + h * a.k_head
-                            : (const RT *)a.q + t * a.q_row + (h - 2 * hkv) * a.q_head;
-    pg_load(src + d0, x);
-    pg_load(src + d1, y);
+                    : h < 2 * hkv ? (const RT *)a.v + t * a.v_row + (h - hkv) * a.v_head
+                                  : (const RT *)a.q + t * a.q_row + (h - 2 * hkv) * a.q_head;
+    turned = c < (a.rotary_dim >> 4) && (h < hkv || h >= 2 * hkv);
+    d0 = 16 * c;
+    d1 = d0 + 8;
+    if (turned && !a.interleaved) d0 = 8 * c, d1 = d0 + (a.rotary_dim >> 1);
+    x.load(src + d0);
+    y.load(src + d1);
+  }
+  template <typename CT>
+  __device__ __forceinline__ void store(const AppendRows &a, int t, int64_t at, const float *cs, const float *sn) const {
+    const int hkv = a.kv.n_kv_heads;
+    float u[8], v[8];
+    x.get(u);
+    y.get(v);
     if (turned) {
+      if (a.interleaved) {  // u holds pairs 8 c .. 8 c + 3, v the next four
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        // interleaved: x holds pairs 8 c .. 8 c + 3, y the next four
-        if (a.interleaved) {
-          if (j & 1) continue;
-          const float c0 = cs[8 * c + j / 2], s0 = sn[8 * c + j / 2];
-          const float c1 = cs[8 * c + 4 + j / 2], s1 = sn[8 * c + 4 + j / 2];
-          const float u = x[j], v = x[j + 1], e = y[j], f = y[j + 1];
-          x[j] = u * c0 - v * s0;
-          x[j + 1] = u * s0 + v * c0;
-          y[j] = e * c1 - f * s1;
-          y[j + 1] = e * s1 + f * c1;
-        } else {
-          const float c0 = cs[8 * c + j], s0 = sn[8 * c + j];
-          const float u = x[j], v = y[j];
-          x[j] = u * c0 - v * s0;
-          y[j] = u * s0 + v * c0;
+        for (int j = 0; j < 8; j += 2) {
+          const float c0 = cs[8 * c + j / 2], s0 = sn[8 * c + j / 2], c1 = cs[8 * c + 4 + j / 2], s1 = sn[8 * c + 4 + j / 2];
+          const float p = u[j], q = u[j + 1], e = v[j], f = v[j + 1];
+          u[j] = p * c0 - q * s0;
+          u[j + 1] = p * s0 + q * c0;
+          v[j] = e * c1 - f * s1;
+          v[j + 1] = e * s1 + f * c1;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const float c0 = cs[8 * c + j], s0 = sn[8 * c + j], p = u[j], q = v[j];
+          u[j] = p * c0 - q * s0;
+          v[j] = p * s0 + q * c0;
         }
       }
     }
-    if (h < hkv) {
-      CT *dst = (CT *)a.kv.k + at + h * a.kv.head_stride;
-      pg_store(dst + d0, x);
-      pg_store(dst + d1, y);
+    if (h < 2 * hkv) {
+      CT *dst = h < hkv ? (CT *)a.kv.k + at + h * a.kv.head_stride : (CT *)a.kv.v + at + (h - hkv) * a.kv.head_stride;
+      pg_store(dst + d0, u);
+      pg_store(dst + d1, v);
     } else {
       RT *dst = (RT *)a.q_out + t * a.o_row + (h - 2 * hkv) * a.o_head;
-      pg_store(dst + d0, x);
-      pg_store(dst + d1, y);
+      pg_store(dst + d0, u);
+      pg_store(dst + d1, v);
     }
+  }
+};
+
+template <typename RT, typename CT>
+__global__ __launch_bounds__(PA_NT) void paged_append_kernel(AppendArgs args) {
+  __shared__ float cs[64], sn[64];
+  const AppendRows rows = args.rows;  // (the angles' table is indexed: by itself, it stays in the arguments)
+  const int t = blockIdx.x, tid = threadIdx.x;
+  const int per = args.head_dim >> 4, chunks = (2 * rows.kv.n_kv_heads + (rows.q ? args.n_heads : 0)) * per;
+  PaChunk<RT> w0, w1;
+  if (tid < chunks) w0.load(rows, t, tid, per);
+  if (tid + PA_NT < chunks) w1.load(rows, t, tid + PA_NT, per);
+  const int p = args.pos[t], s = args.seq ? args.seq[t] : t;
+  if (p < 0 || s < 0 || s >= args.n_seqs) return;
+  const int64_t slot = (int64_t)p - args.base;
+  const int page = pg_page(args.table + (int64_t)s * args.table_stride, args.table_width, slot, rows.kv.page_shift, rows.kv.n_pages);
+  if (page < 0) return;
+  if (tid < rows.rotary_dim >> 1) {
+    const double r = p * args.turns[tid];
+    sincospif(2.0f * (float)(r - rint(r)), &sn[tid], &cs[tid]);
+  }
+  __syncthreads();
+  const int64_t at = page * rows.kv.page_stride + (slot & (rows.kv.page_size - 1)) * rows.kv.token_stride;
+  if (tid < chunks) w0.template store<CT>(rows, t, at, cs, sn);
+  if (tid + PA_NT < chunks) w1.template store<CT>(rows, t, at, cs, sn);
+  for (int i = tid + 2 * PA_NT; i < chunks; i += PA_NT) {
+    w0.load(rows, t, i, per);
+    w0.template store<CT>(rows, t, at, cs, sn);
   }
 }
 
