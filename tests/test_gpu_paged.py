@@ -181,6 +181,28 @@ def test_attend_many_sequences_and_long_contexts(rows, cache):
 
 
 @pytest.mark.parametrize("rows,cache", PAIRS)
+def test_attend_shared_prefix_in_wide_blocks(rows, cache):
+    """More columns than a narrow block takes, over a prefix of several splits
+    that ends inside a page and a step, next to own keys of several splits."""
+    torch.manual_seed(18)
+    n, hkv, hd, page, prefix = 37, 2, 128, 16, 777
+    lens = [int(x) for x in torch.randint(0, 500, (n,))]
+    lens[3], lens[9] = 0, 512
+    width, pre = 32, -(-prefix // page)
+    kp, vp = pools(n * width + pre, hkv, page, hd, TYPES[cache], 19)
+    order = torch.randperm(n * width + pre).to(torch.int32).to(DEV)
+    q = torch.randn(n, 8, hd, device=DEV).to(TYPES[rows]) * 1.5
+    kp[order[n * width + pre - 1].item(), :, prefix % page:] = math.nan
+    vp[order[n * width + pre - 1].item(), :, prefix % page:] = math.nan
+    table = order[:n * width].view(n, width)
+    bad = order[n * width:].clone()
+    check(q, kp, vp, table, ints(lens), prefix_pages=bad, prefix_len=prefix)
+    bad[7] = -1  # a hole of 16 keys
+    bad[8] = 1 << 20
+    check(q, kp, vp, table, ints(lens), prefix_pages=bad, prefix_len=prefix)
+
+
+@pytest.mark.parametrize("rows,cache", PAIRS)
 def test_attend_leaves_what_is_not_its_own(rows, cache):
     """Rows behind the last sequence stay as they were; NaN and infinities in
     slots that no row sees, in pages of nobody and in padding rows change

@@ -5,8 +5,8 @@ that shares a prefix, and sampling.
 
 Arguments are torch tensors of one GPU.  Calls are enqueued on the stream that
 is current for it (`stream`: another one, an object with `cuda_stream` or its
-number; the tensors must then be kept alive, and ready, for that stream by the
-caller) and return without waiting.  They can be captured into graphs.  Wrong
+number; the caller then keeps the arguments alive and ready for that stream,
+and tensors that the call makes belong to it) and return without waiting.  They can be captured into graphs.  Wrong
 shapes, types, strides or devices raise ValueError or TypeError, what the
 library refuses raises VoxtralError.  There is no backward pass: tensors that
 require gradients are refused while gradients are recorded."""
@@ -49,8 +49,17 @@ def _stream(index, stream):
     return _raw_stream(index) if stream is None else getattr(stream, "cuda_stream", stream)
 
 
-def _as_stream(stream, index):
-    return stream if isinstance(stream, _torch.cuda.Stream) else _torch.cuda.ExternalStream(_stream(index, stream), index)
+def _made(stream, index, make):
+    """make()'s tensor for a call on `stream`: memory is taken from that
+    stream's own, since what the current stream has freed it may still be
+    using."""
+    if stream is None:
+        return make()
+    if not isinstance(stream, _torch.cuda.Stream):
+        number = _stream(index, stream)
+        stream = _torch.cuda.ExternalStream(number, index) if number else _torch.cuda.default_stream(index)
+    with _torch.cuda.stream(stream):
+        return make()
 
 
 def _refuse(name, x, dims, index):
@@ -154,7 +163,7 @@ class PagedKV:
             q_at, q_row, q_head = self._rows("q", q, n, None)
             heads = q.shape[1]
             if q_out is None:
-                q_out = q.new_zeros(q.shape)
+                q_out = _made(stream, self.index, lambda: q.new_zeros(q.shape))
             o_at, o_row, o_head = self._rows("q_out", q_out, n, heads)
             if q.dtype != dtype or q_out.dtype != dtype:
                 raise TypeError(f"q is {q.dtype}, q_out is {q_out.dtype}, k is {dtype}")
@@ -193,7 +202,7 @@ class PagedKV:
         if max_len is None:
             max_len = width * self.page_size
         if out is None:
-            out = q.new_empty(q.shape) if row_start is None else q.new_zeros(q.shape)
+            out = _made(stream, index, lambda: q.new_empty(q.shape) if row_start is None else q.new_zeros(q.shape))
         o_at, o_row, o_head = self._rows("out", out, n, heads)
         if out.dtype != q.dtype:
             raise TypeError(f"out is {out.dtype}, q is {q.dtype}")
@@ -213,10 +222,7 @@ class PagedKV:
             need = ctypes.c_size_t()
             _call(self._lib.vx_paged_attend_workspace, _ATTEND.pack(*args), ctypes.byref(need))
             if need.value:
-                # torch's allocator orders its reuse by the current stream
-                workspace = table.new_empty((need.value + 3) // 4)
-                if stream is not None:
-                    workspace.record_stream(_as_stream(stream, index))
+                workspace = _made(stream, index, lambda: table.new_empty((need.value + 3) // 4))
         else:
             _tensor("workspace", workspace, 1, index)
         if workspace is not None:
@@ -266,9 +272,8 @@ def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=N
         m_at, min_p = _vector("min_p", min_p, f32, rows, index), 0
     u_at = _vector("u", u, _torch.float64, rows, index)
     if out is None:
-        token = logits.new_empty(rows, dtype=i32)
-        kept = logits.new_empty(rows, dtype=i32)
-        prob = logits.new_empty(rows, dtype=f32)
+        token, kept, prob = _made(stream, index, lambda: (logits.new_empty(rows, dtype=i32), logits.new_empty(rows, dtype=i32),
+                                                          logits.new_empty(rows, dtype=f32)))
         at = token.data_ptr(), kept.data_ptr(), prob.data_ptr()
     else:
         token, kept, prob = out
@@ -278,10 +283,8 @@ def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=N
     space = _sample_space(lib, rows, n, kind, index)
     work = 0
     if space:
-        work = logits.new_empty((space + 3) // 4, dtype=i32)
-        if stream is not None:
-            work.record_stream(_as_stream(stream, index))
-        work = work.data_ptr()
+        held = _made(stream, index, lambda: logits.new_empty((space + 3) // 4, dtype=i32))
+        work = held.data_ptr()
     _call(lib.vx_sample_rows, _SAMPLE.pack(logits.data_ptr(), logits.stride(0), t_at, p_at, m_at, k_at, u_at, *at, rows, n, kind, index,
                                            temperature, top_p, min_p, top_k, work, space), _stream(index, stream))
     return token, kept, prob
