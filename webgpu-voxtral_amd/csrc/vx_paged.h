@@ -118,7 +118,8 @@ constexpr int PA_NT = 256;
 // those of the two halves of a pair when pairs are (i, i + rotary_dim / 2).
 // Bound by memory where there are many tokens, by latency where there are few:
 // the first two chunks are asked for before the token's page and angles are
-// known.
+// known (3908 f16 tokens of 32 + 8 + 8 heads, 94 MB: 30 -> 22.5 us = 4.2 TB/s;
+// 8 tokens 5.1 -> 4.0 us).
 template <typename RT>
 struct PaChunk {
   int h, c, d0, d1;  // head (keys, values, queries), chunk, its elements' places
@@ -221,7 +222,14 @@ __global__ __launch_bounds__(PA_NT) void paged_append_kernel(AppendArgs args) {
 // bound by HBM: the matrix cores are all but idle.  Many columns (wide): the
 // waves bring 128 keys together through LDS, laid out as the matrix
 // instruction's operands, and each takes 32 columns (16 for f32 rows) through
-// all of them.
+// all of them.  64 columns is where the two meet: a prefix of 2050 keys for 256
+// columns a KV head takes 26-32 us in narrow blocks (each of four waves reads
+// every key, and their partials are many) and 19 us in wide ones, and 1500 keys
+// for 3520 columns 122 and 47 us.
+//
+// Measured: 64 sequences of 512 own keys (f16, 134 MB) 26.4 us = 5.1 TB/s, 32
+// of 8192 (1.07 GB) 181 us = 5.9 TB/s; 64 of 200-900 behind 2050 shared keys
+// 39.5 us and 5.3 for the join.
 struct AttendArgs {
   PagedKV kv;
   const void *q;
@@ -284,6 +292,10 @@ inline AttendPlan attend_plan(int n_rows, int n_seqs, int n_heads, int n_kv_head
   };
   choose(cols, &p.pre_cols, &p.pre_wide);
   choose(ragged ? cols / (n_seqs > 0 ? n_seqs : 1) : g, &p.own_cols, &p.own_wide);
+  // Fused where the prefix costs less than a launch of the join: in wide blocks
+  // (its keys serve 128 columns of the sequence as well as of others: 85 us
+  // against 85 + 18 at 16 prompts behind 1500 keys), and where all keys are at
+  // most 512 (4 x 1-40 behind 100: 8.4 us against 7.0 + 3.5).
   p.fused = prefix_len > 0 && max_len > 0 && (p.own_wide || (int64_t)prefix_len + max_len <= 512);
   if (prefix_len > 0 && !p.fused) {
     p.pre_tiles = (int)at_ceil(cols, p.pre_cols);
@@ -297,6 +309,7 @@ inline AttendPlan attend_plan(int n_rows, int n_seqs, int n_heads, int n_kv_head
           p.fused && !p.own_wide ? 1 : p.own_wide ? cus : 3 * cus, &p.own_splits, &p.own_chunk);
   }
   const int64_t items = p.direct() ? 0 : (int64_t)p.slots() * n_rows * n_heads;
+  // a block joins one item's partials instead of four where they are many
   p.team = p.slots() >= 24 ? AT_WAVES : 1;
   p.ml_at = (size_t)items * head_dim * 4;
   p.bytes = p.ml_at + (size_t)items * 8;
@@ -717,7 +730,9 @@ struct AtLds {
   uint32_t rows[AT_WAVES];  // of each step of the stage: what clean() returned
 };
 
-// Few columns: 16 a wave; waves with the same ones split the keys
+// Few columns: 16 a wave; waves with the same ones split the keys.  Asking one
+// step ahead took 24 sequences on an f32 cache from 35 to 25 us; steps of 16
+// keys there (as many bytes in flight, half the registers) to 23.
 template <typename RT, typename CT, int HD>
 __device__ __forceinline__ void at_narrow(const AttendArgs &a, const AtJob &b, int cols, int kvh, u32x4 *so,
                                           float (*sm)[64], float (*sl)[64]) {
@@ -818,7 +833,9 @@ __device__ __forceinline__ void at_narrow(const AttendArgs &a, const AtJob &b, i
 }
 
 // Many columns: a stage is 128 keys, 32 brought by each wave, and every wave
-// takes them all through its own columns
+// takes them all through its own columns.  16 prompts of 20-90 rows behind 1500
+// keys (27.5 GFLOP, bf16): 153 us in narrow blocks, 89 in wide ones with the
+// prefix before each sequence's own keys and nothing to join.
 template <typename RT, typename CT, int HD>
 __device__ __forceinline__ void at_wide(const AttendArgs &a, const AtJob &b, int kvh, AtLds<RT, CT, HD, true> &s) {
   using Y = AtTypes<RT, CT, HD>;

@@ -18,6 +18,13 @@
 // hold more entries than the list (long runs of equal values), the
 // cuts are looked for one after the other, the bin being narrowed by digits
 // of (value, index) first.
+//
+// Bound by LDS additions and weights (two additions and some 30 instructions an
+// entry) where rows are long, by the latency of about a dozen barriers where
+// they are short.  A row of 8320 f32 logits takes 15.4 us in one block (load 2,
+// range 2, bins 3, cuts 4, gathering and places 4), 64 of them 19; 256 of
+// 131072 f32 91 us in a block each (134 MB: 1.5 TB/s); 8 of them, 16 blocks
+// each, 41 us in four launches against 129 in a block each.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -804,7 +811,8 @@ __global__ __launch_bounds__(SR_NT) void sample_rows_kernel(SampleArgs a) {
 // A block a row of 16-bit logits: a pass counts how often each of the 65536
 // values occurs, which is one LDS addition an entry; everything up to the
 // draw then goes by values and their numbers, with one weight a value.  A
-// second pass finds the entry among those of the drawn value.
+// second pass finds the entry among those of the drawn value.  256 rows of
+// 131072 bf16: 44 us (first pass 13, second 9), against 117 by bins.
 // Values by falling order: the bit pattern at a place (0: the largest).
 __device__ __forceinline__ uint32_t sr_place_bits(uint32_t place) { return place < 0x8000u ? 0x7fffu - place : place; }
 template <typename T>
