@@ -418,7 +418,9 @@ int vx_paged_append(const vx_append_args *a, void *stream);
  * of exponentials.  max_len: a bound on lens that the host knows, at most
  * table_width * page_size; work is dealt out by it.  Scores, softmax and sums
  * are f32; with 16-bit rows the weights are rounded to the cache's type
- * before they meet the values. */
+ * before they meet the values, and products of f32 rows with an f16 cache are
+ * good to 2^-21.  At most 2^18 rows, 2^18 sequences and 2^28
+ * keys of a list. */
 typedef struct vx_attend_args {
   vx_paged_kv kv;
   const void *q;                           /* [n_rows][n_heads][head_dim] */
@@ -455,7 +457,10 @@ int vx_paged_attend_workspace(const vx_attend_args *a, size_t *bytes);
  * on the order of sums.  kept and prob (nullable) receive the number of kept
  * entries and the drawn one's share of their weights.  A row with nothing to
  * draw gives token -1, kept 0, prob 0.  Each of temperature, top_k, top_p,
- * min_p is [rows] on the device, or NULL for the same value in every row. */
+ * min_p is [rows] on the device, or NULL for the same value in every row.
+ * Values on the device that are out of range: top_p at most 0 keeps one
+ * entry, min_p above 1 acts as 1, NaN turns a truncation off, and makes the
+ * choice greedy (temperature) or the first entry (u). */
 typedef struct vx_sample_args {
   const void *logits;                      /* [rows][n] */
   int64_t row_stride;

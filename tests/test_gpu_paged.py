@@ -398,6 +398,8 @@ def test_refusals_of_tensors():
             (ValueError, "gradient", lambda: kv.attend(q.clone().requires_grad_(), lens, table)),
             (V.VoxtralError, "multiples of 16", lambda: kv.attend(torch.zeros(2, 4, 65, device=DEV).half()[..., :64], lens, table)),
             (ValueError, "lse", lambda: kv.attend(q, lens, table, lse=torch.zeros(2, 4, device=DEV).half())),
+            (ValueError, "out of range", lambda: kv.attend(q, lens, table, max_len=1 << 40)),
+            (ValueError, "out of range", lambda: kv.append(k, k, lens, table, base=1 << 31)),
             (TypeError, "v is", lambda: kv.append(k, k.float(), lens, table)),
             (V.VoxtralError, "rotary_dim 24", lambda: kv.append(k, k, lens, table, rotary_dim=24)),
             (V.VoxtralError, "theta", lambda: kv.append(k, k, lens, table, theta=-1.0)),

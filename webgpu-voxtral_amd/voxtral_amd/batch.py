@@ -39,6 +39,13 @@ def _load():
     return load_library()
 
 
+def _pack(layout, *args):
+    try:
+        return layout.pack(*args)
+    except struct.error as e:  # a number that its field does not hold
+        raise ValueError(f"an argument is out of range: {e}") from None
+
+
 def _call(fn, *args):
     rc = fn(*args)
     if rc != VX_OK:
@@ -70,7 +77,7 @@ def _refuse(name, x, dims, index):
         raise ValueError(f"{name} is on {x.device}, not on GPU {index}")
     if x.dim() != dims:
         raise ValueError(f"{name} has {x.dim()} dimensions, not {dims}")
-    if x.requires_grad:
+    if x.requires_grad and _torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: this operator has no backward pass")
     raise ValueError(f"{name}: the last dimension is not contiguous")
 
@@ -169,10 +176,10 @@ class PagedKV:
                 raise TypeError(f"q is {q.dtype}, q_out is {q_out.dtype}, k is {dtype}")
         i32 = self._int32
         _call(self._lib.vx_paged_append,
-              _APPEND.pack(self._head, k_at, v_at, k_row, k_head, v_row, v_head, q_at, o_at, q_row, q_head, o_row, o_head,
-                           _vector("pos", pos, i32, n, self.index), 0 if seq is None else _vector("seq", seq, i32, n, self.index),
-                           table_at, table_row, width, base, n, seqs, heads, _types[dtype], theta,
-                           self.head_dim if rotary_dim is None else rotary_dim, bool(interleaved)), _stream(self.index, stream))
+              _pack(_APPEND, self._head, k_at, v_at, k_row, k_head, v_row, v_head, q_at, o_at, q_row, q_head, o_row, o_head,
+                    _vector("pos", pos, i32, n, self.index), 0 if seq is None else _vector("seq", seq, i32, n, self.index),
+                    table_at, table_row, width, base, n, seqs, heads, _types[dtype], theta,
+                    self.head_dim if rotary_dim is None else rotary_dim, bool(interleaved)), _stream(self.index, stream))
         return q_out if q is not None else None
 
     def attend(self, q, lens, table, row_start=None, prefix_pages=None, prefix_len=0, max_len=None, scale=None, out=None,
@@ -220,14 +227,14 @@ class PagedKV:
                 prefix_len, max_len, n, seqs, heads, _types[q.dtype], scale, 0, 0]
         if workspace is None:
             need = ctypes.c_size_t()
-            _call(self._lib.vx_paged_attend_workspace, _ATTEND.pack(*args), ctypes.byref(need))
+            _call(self._lib.vx_paged_attend_workspace, _pack(_ATTEND, *args), ctypes.byref(need))
             if need.value:
                 workspace = _made(stream, index, lambda: table.new_empty((need.value + 3) // 4))
         else:
             _tensor("workspace", workspace, 1, index)
         if workspace is not None:
             args[-2], args[-1] = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        _call(self._lib.vx_paged_attend, _ATTEND.pack(*args), _stream(index, stream))
+        _call(self._lib.vx_paged_attend, _pack(_ATTEND, *args), _stream(index, stream))
         return out
 
     def attend_workspace(self, rows, heads, seqs, width, ragged=False, prefix_len=0, max_len=None, dtype=None):
@@ -235,9 +242,9 @@ class PagedKV:
         `heads` heads, a table of seqs x width pages and these bounds."""
         need = ctypes.c_size_t()
         t = _types[self.k_pages.dtype if dtype is None else dtype]
-        args = _ATTEND.pack(self._head, 0, 0, 0, 0, 0, 0, 0, int(ragged), 0, 0, 0, width, width,
-                            -(-prefix_len // self.page_size), prefix_len, width * self.page_size if max_len is None else max_len,
-                            rows, seqs, heads, t, 0.0, 0, 0)
+        args = _pack(_ATTEND, self._head, 0, 0, 0, 0, 0, 0, 0, int(ragged), 0, 0, 0, width, width,
+                     -(-prefix_len // self.page_size), prefix_len, width * self.page_size if max_len is None else max_len,
+                     rows, seqs, heads, t, 0.0, 0, 0)
         _call(self._lib.vx_paged_attend_workspace, args, ctypes.byref(need))
         return need.value
 
@@ -285,8 +292,8 @@ def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=N
     if space:
         held = _made(stream, index, lambda: logits.new_empty((space + 3) // 4, dtype=i32))
         work = held.data_ptr()
-    _call(lib.vx_sample_rows, _SAMPLE.pack(logits.data_ptr(), logits.stride(0), t_at, p_at, m_at, k_at, u_at, *at, rows, n, kind, index,
-                                           temperature, top_p, min_p, top_k, work, space), _stream(index, stream))
+    _call(lib.vx_sample_rows, _pack(_SAMPLE, logits.data_ptr(), logits.stride(0), t_at, p_at, m_at, k_at, u_at, *at, rows, n, kind, index,
+                                   temperature, top_p, min_p, top_k, work, space), _stream(index, stream))
     return token, kept, prob
 
 
